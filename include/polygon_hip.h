@@ -189,6 +189,54 @@ PG_API int pg_sample_forced(const pg_dims* d, int dtype, const float* params, co
                             float temp, int multinomial, uint8_t* tokens, int32_t* end_pads, const uint8_t* forced,
                             float* probs_out, void* stream);
 
+/* ---- Beam search (no counterpart in the reference, whose decoder only draws or takes the argmax, vae_model.py:300-358) ----
+ *
+ * pg_beam_select: one step of the selection over K beams and V symbols, for n independent groups (molecules).
+ *   x = logits[g, k, v] where allowed (mask), m = max_v x, Z = sum_v exp((x - m) / temp)      (64-bit arithmetic)
+ *   logp = fp32((x - m) / temp - log Z);   c = fp32(scores[g, k] + logp)
+ * and the K largest c > -inf of the group's K * V, equal ones by the lower k * V + v.  A beam whose finished flag is set has
+ * one candidate, (pad, its own score), and its logits are not read; a beam whose score is not finite, or whose allowed logits
+ * hold a NaN, a +inf or nothing above -inf, has none.  Each entry gets its score, the beam it continues (parents), its symbol
+ * and finished = parent's flag or symbol == eos (eos < 0: never).  Where fewer than K candidates exist the rest are: score
+ * -inf, symbol pad, finished, parent = the entry's own place.
+ * Order: keep_slots = 0: by rank.  keep_slots = 1: the best child of each beam keeps that beam's place, the others take the
+ * places of beams without a child (ascending, by rank), so that a state moves only where parents[j] != j and a place that is
+ * read by another is never itself overwritten.
+ * logits: dtype, element (g, k, v) at g * ld_group + k * ld_row + v.  mask (nullable): bytes, 0 = forbidden, element (g, k, v)
+ * at g * mask_group + k * mask_row + v (0 strides share one mask).  scores_out / finished_out may be scores / finished.
+ * K <= PG_MAX_BEAMS, V <= PG_MAX_BEAM_V.  ws: pg_beam_select_workspace_bytes (0 for short vocabularies: ws may be NULL). */
+#define PG_MAX_BEAMS 32
+#define PG_MAX_BEAM_V (1 << 20)
+PG_API size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V);
+PG_API int pg_beam_select(int dtype, const void* logits, long ld_group, long ld_row, int n, int K, int V, const uint8_t* mask,
+                          long mask_group, long mask_row, double temp, const float* scores, const uint8_t* finished, int eos,
+                          int pad, int keep_slots, float* scores_out, int32_t* parents, int32_t* tokens, uint8_t* finished_out,
+                          void* ws, size_t ws_bytes, void* stream);
+
+/* Pages of a cache of decoder states.  A cache is n_planes arrays ("planes", e.g. the fp32 state and the operand copy of every
+ * layer); page p is row p of every plane: `bytes` bytes at base + p * pitch.  Any width, pitch and alignment is taken; planes
+ * of one call may interleave in one buffer but not share bytes (refused).  Indices live on the device and are checked by the
+ * kernels: one that is out of range moves nothing.  Bytes outside the pages named are left as they are. */
+#define PG_MAX_PLANES 32
+typedef struct pg_plane {
+  void* base;
+  long pitch, bytes;
+} pg_plane;
+
+/* pg_pages_reorder: pages g*K .. g*K+K-1 are group g's; page g*K + j takes over the contents that page g*K + parents[g*K + j]
+ * had before the call (any parents, in place).  Pages with parents == j are neither read nor written unless another needs them.
+ * pg_pages_fork: page i of dst = page index[i] of src, for i < n_dst (copies and forks; an index may occur any number of
+ * times).  dst[i].bytes == src[i].bytes; dst and src share no bytes.
+ * pg_pages_compact: in place; count[0] = number of live pages (live[p] != 0); live pages at or behind count move, in ascending
+ * order, to the dead places below it.  map[p] = the new place of old page p, -1 if it was freed.  Contents of pages at or
+ * behind count are left as they were.  ws: pg_pages_compact_workspace_bytes. */
+PG_API int pg_pages_reorder(const pg_plane* planes, int n_planes, int n_groups, int K, const int32_t* parents, void* stream);
+PG_API int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_planes, int n_dst, int n_src, const int32_t* index,
+                         void* stream);
+PG_API size_t pg_pages_compact_workspace_bytes(int n_pages);
+PG_API int pg_pages_compact(const pg_plane* planes, int n_planes, int n_pages, const uint8_t* live, int32_t* count, int32_t* map,
+                            void* ws, size_t ws_bytes, void* stream);
+
 /* Parity hook (no reference counterpart; HOST function, touches no GPU): the inter-layer dropout masks that
  * pg_decoder_fwd / pg_decoder_bwd apply for (seed, p_drop, pg_dp.b_mul/b_add), computed by the same inline function the
  * kernels call.  out (host memory) float [n_masks, B, T, H]: mask of layer l's output at decoder step t of local row b,

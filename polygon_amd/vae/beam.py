@@ -1,0 +1,196 @@
+"""Operators of beam search on the device: the selection over beams and vocabulary, and the moves of the decoder states that
+follow it (pg_beam_select, pg_pages_reorder, pg_pages_fork, pg_pages_compact of include/polygon_hip.h).  ``VAE.beam_search``
+runs the whole decode; these serve a program that drives its own.
+
+All work is enqueued on the current stream of the tensors' device; nothing synchronises or copies to the host.  Arguments are
+checked on the host (shapes, types, devices, strides); indices are device data and checked by the kernels: one that is out of
+range moves nothing.  Nothing here is differentiable.
+"""
+import ctypes
+from typing import NamedTuple
+
+import torch
+
+from polygon_amd import _lib
+
+MAX_BEAMS = 32      # PG_MAX_BEAMS
+
+
+class _Plane(ctypes.Structure):
+    _fields_ = [("base", ctypes.c_void_p), ("pitch", ctypes.c_long), ("bytes", ctypes.c_long)]
+
+
+class BeamStep(NamedTuple):
+    """One step of the selection, every member [n, K] and indexed by the place a beam now has."""
+    scores: torch.Tensor        # float32: sum of the log-probabilities, -inf where there was no candidate
+    parents: torch.Tensor       # int32: the place, before the step, of the beam this one continues
+    tokens: torch.Tensor        # int32: the symbol appended to it
+    finished: torch.Tensor      # bool
+
+
+_entry = None
+
+
+def _entries():
+    """The library's entry points with their argument types declared once (ctypes then converts plain ints by itself)."""
+    global _entry
+    if _entry is None:
+        L = _lib.lib()
+        i, l, p, z, d = ctypes.c_int, ctypes.c_long, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_double
+        L.pg_beam_select.argtypes = [i, p, l, l, i, i, i, p, l, l, d, p, p, i, i, i, p, p, p, p, p, z, p]
+        L.pg_beam_select_workspace_bytes.argtypes, L.pg_beam_select_workspace_bytes.restype = [i, i, i, i], z
+        L.pg_pages_reorder.argtypes = [p, i, i, i, p, p]
+        L.pg_pages_fork.argtypes = [p, p, i, i, i, p, p]
+        L.pg_pages_compact.argtypes = [p, i, i, p, p, p, p, z, p]
+        L.pg_pages_compact_workspace_bytes.argtypes, L.pg_pages_compact_workspace_bytes.restype = [i], z
+        _entry = L
+    return _entry
+
+
+class _On:
+    """Makes ``device`` the current one for the length of a call (nothing to do where it is) and knows its current stream."""
+
+    def __init__(self, device):
+        if device.type != "cuda":
+            raise _lib.PolygonHipError("polygon_amd computes only on an MI355X (`cuda`) device, got a tensor on %s" % device)
+        self.device, self.before = device, torch.cuda.current_device()
+
+    def __enter__(self):
+        if self.device.index != self.before:
+            torch.cuda.set_device(self.device)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.device.index != self.before:
+            torch.cuda.set_device(self.before)
+
+
+def _flags(t, shape, device, what):
+    if t.dtype not in (torch.bool, torch.uint8):
+        raise ValueError("%s must be bool or uint8, got %s" % (what, t.dtype))
+    if tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError("%s must be %s on %s, got %s on %s" % (what, list(shape), device, list(t.shape), t.device))
+    return t.contiguous()
+
+
+def beam_select(logits, scores, finished=None, mask=None, temp=1.0, eos=-1, pad=0, keep_slots=False) -> BeamStep:
+    """The K best of the K * V continuations of every group's K beams.
+
+    ``logits`` [n, K, V] float32 or bfloat16 (any strides; the last dimension is copied if it is not dense), ``scores`` [n, K]
+    float32 (-inf: a place without a beam), ``finished`` [n, K] bool (a finished beam competes with its own score and appends
+    ``pad``), ``mask`` [V], [K, V], [n, 1, V] or [n, K, V] bool (False: the symbol is left out, also of the normaliser; what
+    the logits hold there is not looked at).  A candidate's score is scores + log_softmax(logits / temp) with the normaliser in
+    64 bits; equal scores go by the lower k * V + v.  ``eos`` (-1: none) finishes a beam.  K <= 32, V <= 2**20.
+
+    ``keep_slots``: the best child of a beam stays in that beam's place and the others take the places that became free,
+    instead of the order by rank: then ``reorder_pages`` moves only the states of beams with more than one child."""
+    if logits.dim() != 3 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be [n, K, V] float32 or bfloat16, got %s %s" % (list(logits.shape), logits.dtype))
+    n, K, V = logits.shape
+    dev = logits.device
+    if tuple(scores.shape) != (n, K) or scores.dtype != torch.float32 or scores.device != dev:
+        raise ValueError("scores must be [%d, %d] float32 on %s, got %s %s on %s" % (n, K, dev, list(scores.shape), scores.dtype,
+                                                                                  scores.device))
+    with _On(dev) as stream:
+        L = _entries()
+        if V > 1 and logits.stride(2) != 1:
+            logits = logits.contiguous()
+        scores = scores.contiguous()
+        if finished is not None:
+            finished = _flags(finished, (n, K), dev, "finished")
+        mg = mr = 0
+        if mask is not None:
+            if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev:
+                raise ValueError("mask must be bool or uint8 on %s, got %s on %s" % (dev, mask.dtype, mask.device))
+            if not 1 <= mask.dim() <= 3 or any(a not in (1, b) for a, b in zip(mask.shape[:-1], (n, K)[3 - mask.dim():])) \
+                    or mask.shape[-1] != V:
+                raise ValueError("mask %s does not fit logits %s" % (list(mask.shape), list(logits.shape)))
+            if V > 1 and mask.stride(-1) != 1:
+                mask = mask.contiguous()
+            if mask.dim() > 1 and mask.shape[-2] > 1:
+                mr = mask.stride(-2)
+            if mask.dim() > 2 and mask.shape[0] > 1:
+                mg = mask.stride(0)
+        out = BeamStep(torch.empty(n, K, device=dev), torch.empty(n, K, device=dev, dtype=torch.int32),
+                       torch.empty(n, K, device=dev, dtype=torch.int32), torch.empty(n, K, device=dev, dtype=torch.bool))
+        code = _lib.PG_F32 if logits.dtype == torch.float32 else _lib.PG_BF16
+        need = L.pg_beam_select_workspace_bytes(code, n, K, V)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        _lib.check(L.pg_beam_select(code, logits.data_ptr(), logits.stride(0), logits.stride(1), n, K, V,
+                                    None if mask is None else mask.data_ptr(), mg, mr, float(temp), scores.data_ptr(),
+                                    None if finished is None else finished.data_ptr(), int(eos), int(pad), int(bool(keep_slots)),
+                                    out.scores.data_ptr(), out.parents.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(),
+                                    None if ws is None else ws.data_ptr(), need, stream), "pg_beam_select")
+    return out
+
+
+def _planes(planes, what, pages=None):
+    """The C description of a cache: its planes' first dimension counts pages, what is behind it is one page's dense row."""
+    if not planes:
+        raise ValueError("%s: no planes" % what)
+    out = (_Plane * len(planes))()
+    dev, P = planes[0].device, planes[0].shape[0] if planes[0].dim() else -1
+    for d, t in zip(out, planes):
+        if t.dim() < 1 or t.shape[0] != P or t.device != dev:
+            raise ValueError("%s: every plane must have the same number of pages in front, on one device" % what)
+        if t.requires_grad:
+            raise ValueError("%s: pages are moved in place, a plane must not require gradients" % what)
+        row = t.element_size()
+        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if size != 1 and stride * t.element_size() != row:
+                raise ValueError("%s: what is behind a plane's first dimension must be dense, got strides %s" % (what, list(t.stride())))
+            row *= size
+        if row == 0:
+            raise ValueError("%s: a page of no bytes" % what)
+        d.base, d.bytes = t.data_ptr(), row
+        d.pitch = t.stride(0) * t.element_size() if P > 1 else row
+    return out, dev, P
+
+
+def _index(t, dev, what):
+    if t.dtype != torch.int32 or t.device != dev:
+        raise ValueError("%s must be int32 on %s, got %s on %s" % (what, dev, t.dtype, t.device))
+    return t.contiguous()
+
+
+def reorder_pages(planes, parents):
+    """In place: page g*K + j of every plane takes over what page g*K + parents[g, j] held before the call.  ``planes``:
+    tensors [n*K, ...], dense behind the first dimension; ``parents`` [n, K] int32 (``BeamStep.parents``)."""
+    d, dev, P = _planes(planes, "reorder_pages")
+    if parents.dim() != 2 or parents.shape[0] * parents.shape[1] != P:
+        raise ValueError("parents %s does not name %d pages" % (list(parents.shape), P))
+    parents = _index(parents, dev, "parents")
+    with _On(dev) as stream:
+        _lib.check(_entries().pg_pages_reorder(d, len(planes), parents.shape[0], parents.shape[1], parents.data_ptr(), stream),
+                   "pg_pages_reorder")
+
+
+def fork_pages(dst, src, index):
+    """Page i of ``dst`` becomes a copy of page index[i] of ``src`` in every plane (index int32 [n_dst]; a page may be taken any
+    number of times; a negative index or one behind the last page leaves page i as it is).  dst and src share no memory."""
+    d, dev, P = _planes(dst, "fork_pages: dst")
+    s, sdev, Q = _planes(src, "fork_pages: src")
+    if len(dst) != len(src) or sdev != dev or any(a.dtype != b.dtype or a.shape[1:] != b.shape[1:] for a, b in zip(dst, src)):
+        raise ValueError("fork_pages: dst and src must have the same planes but for the number of pages")
+    if tuple(index.shape) != (P,):
+        raise ValueError("index %s does not name a page for each of %d" % (list(index.shape), P))
+    index = _index(index, dev, "index")
+    with _On(dev) as stream:
+        _lib.check(_entries().pg_pages_fork(d, s, len(dst), P, Q, index.data_ptr(), stream), "pg_pages_fork")
+
+
+def compact_pages(planes, live):
+    """Frees the pages whose ``live`` flag ([P] bool) is not set and closes the gaps, in place: the live pages behind the new
+    end move, in order, to the dead places before it.  Returns (count int32 [1], map int32 [P]: the new place of every old
+    page, -1 for a freed one), both on the device."""
+    d, dev, P = _planes(planes, "compact_pages")
+    live = _flags(live, (P,), dev, "live")
+    with _On(dev) as stream:
+        L = _entries()
+        count = torch.empty(1, device=dev, dtype=torch.int32)
+        where = torch.empty(P, device=dev, dtype=torch.int32)
+        need = L.pg_pages_compact_workspace_bytes(P)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        _lib.check(L.pg_pages_compact(d, len(planes), P, live.data_ptr(), count.data_ptr(), where.data_ptr(), ws.data_ptr(), need,
+                                      stream), "pg_pages_compact")
+    return count, where

@@ -1,0 +1,106 @@
+"""Refusals of the beam-search operators: what the C entries and the Python wrappers turn down on the host, before any kernel
+could see it.  No GPU needed."""
+import ctypes
+
+import pytest
+import torch
+
+from polygon_amd import _lib, vae
+from polygon_amd.vae import beam
+
+FAKE = 1 << 20        # an address that nothing reads: every call below ends at its checks
+
+
+def _select(**kw):
+    a = dict(dtype=_lib.PG_F32, logits=FAKE, ld_group=8, ld_row=4, n=1, K=2, V=4, mask=None, mask_group=0, mask_row=0, temp=1.0,
+             scores=FAKE, finished=None, eos=-1, pad=0, keep=0, scores_out=FAKE, parents=FAKE, tokens=FAKE, finished_out=FAKE,
+             ws=None, ws_bytes=0, stream=None)
+    a.update(kw)
+    return beam._entries().pg_beam_select(*a.values())
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=7), dict(n=-1), dict(K=0), dict(K=33), dict(V=0), dict(V=(1 << 20) + 1), dict(temp=0.0), dict(temp=-1.0),
+    dict(temp=float("nan")), dict(temp=float("inf")), dict(temp=1e-320), dict(pad=-1), dict(pad=4), dict(eos=4), dict(logits=None),
+    dict(scores=None), dict(scores_out=None), dict(parents=None), dict(tokens=None), dict(finished_out=None)])
+def test_select_refuses(kw):
+    assert _select(**kw) == -1
+    assert b"pg_beam_select" in _lib.lib().pg_last_error()
+
+
+def test_select_of_no_group_is_nothing():
+    assert _select(n=0, logits=None, scores=None) == 0
+
+
+def _pl(*rows):
+    out = (beam._Plane * len(rows))()
+    for d, (base, pitch, size) in zip(out, rows):
+        d.base, d.pitch, d.bytes = base, pitch, size
+    return out
+
+
+ONE = (FAKE, 64, 64)
+
+
+def test_pages_refuse():
+    L = beam._entries()
+    reorder = lambda rows, n=2, K=2, par=FAKE, np=None: L.pg_pages_reorder(_pl(*rows), len(rows) if np is None else np, n, K, par, None)  # noqa: E731
+    assert reorder([ONE], n=-1) == reorder([ONE], K=0) == reorder([ONE], K=33) == reorder([ONE], par=None) == -1
+    assert reorder([ONE], np=0) == reorder([ONE], np=33) == L.pg_pages_reorder(None, 1, 2, 2, FAKE, None) == -1
+    assert reorder([(None, 64, 64)]) == reorder([(FAKE, 63, 64)]) == reorder([(FAKE, 64, 0)]) == -1
+    assert reorder([ONE, ONE]) == -1 and b"share" in L.pg_last_error()
+    assert reorder([ONE, (FAKE + 32, 64, 64)]) == -1
+    assert reorder([(FAKE, 128, 64), (FAKE + 63, 128, 64)]) == -1          # interleaved, one byte in common
+    assert reorder([(FAKE, 128, 64), (FAKE + 64, 128, 65)]) == -1          # runs into the next row of the first
+    assert reorder([ONE], n=0, par=None) == 0
+
+    fork = lambda d, s, nd=4, ns=4, idx=FAKE: L.pg_pages_fork(_pl(d), _pl(s), 1, nd, ns, idx, None)  # noqa: E731
+    far = (FAKE + (1 << 16), 64, 64)
+    assert fork(ONE, ONE) == fork(ONE, (FAKE + 192, 64, 64)) == -1         # the last page of dst is the first of src
+    assert fork(ONE, (FAKE + (1 << 16), 64, 32)) == fork(ONE, (FAKE + (1 << 16), 16, 64)) == fork(ONE, (None, 64, 64)) == -1
+    assert fork(ONE, far, nd=-1) == fork(ONE, far, ns=-1) == fork(ONE, far, idx=None) == -1
+    assert L.pg_pages_fork(_pl(ONE), None, 1, 4, 4, FAKE, None) == -1
+    assert fork(ONE, far, nd=0, idx=None) == fork(ONE, far, ns=0, idx=None) == 0
+
+    need = L.pg_pages_compact_workspace_bytes(4)
+    compact = lambda n=4, live=FAKE, count=FAKE, m=FAKE, ws=FAKE, size=need: L.pg_pages_compact(_pl(ONE), 1, n, live, count, m, ws, size, None)  # noqa: E731
+    assert compact(n=-1) == compact(live=None) == compact(count=None) == compact(m=None) == -1
+    assert compact(ws=None) == compact(size=need - 1) == -4
+
+
+def test_interleaved_planes_are_told_from_shared_ones():
+    """planes of one buffer: columns [0, 64) and [64, 128) of rows of 128 bytes share nothing, whichever comes first"""
+    L = beam._entries()
+    a, b = (FAKE, 128, 64), (FAKE + 64, 128, 64)
+    assert L.pg_pages_fork(_pl(a), _pl(b), 1, 0, 4, None, None) == 0
+    for d, s in ((a, b), (b, a)):      # passes the planes' checks and stops at the missing index
+        assert L.pg_pages_fork(_pl(d), _pl(s), 1, 4, 4, None, None) == -1 and b"index" in L.pg_last_error()
+
+
+def test_wrappers_refuse():
+    x, s = torch.zeros(2, 3, 5), torch.zeros(2, 3)
+    with pytest.raises(_lib.PolygonHipError):
+        vae.beam_select(x, s)                                              # not on the GPU
+    for bad in (dict(logits=x[0]), dict(logits=x.double()), dict(logits=x.half()), dict(scores=s[:1]), dict(scores=s.double())):
+        with pytest.raises(ValueError):
+            vae.beam_select(**dict(dict(logits=x, scores=s), **bad))
+    pages, par = torch.zeros(6, 4), torch.zeros(2, 3, dtype=torch.int32)
+    with pytest.raises(_lib.PolygonHipError):
+        vae.reorder_pages([pages], par)
+    for planes, parents in (([], par), ([pages[:5]], par), ([pages.t()], par[:, :2]), ([pages, pages[:5]], par), ([pages], par.long()),
+                            ([pages], par.reshape(-1)), ([pages.clone().requires_grad_()], par), ([torch.zeros(6, 0)], par),
+                            ([torch.zeros(6, 4, 4).transpose(1, 2)], par), ([torch.tensor(1.0)], par)):
+        with pytest.raises(ValueError):
+            vae.reorder_pages(planes, parents)
+    idx = torch.zeros(6, dtype=torch.int32)
+    for dst, src, index in (([pages], [pages[:, :3]], idx), ([pages], [pages.double()], idx), ([pages], [pages, pages], idx),
+                            ([pages], [pages], idx[:5]), ([pages], [pages], idx.long())):
+        with pytest.raises(ValueError):
+            vae.fork_pages(dst, src, index)
+    for live in (torch.zeros(5, dtype=torch.bool), torch.zeros(6)):
+        with pytest.raises(ValueError):
+            vae.compact_pages([pages], live)
+
+
+def test_structs_match_the_header():
+    assert ctypes.sizeof(beam._Plane) == 24 and beam.MAX_BEAMS == 32
