@@ -229,7 +229,7 @@ typedef struct pg_plane {
  * times).  dst[i].bytes == src[i].bytes; dst and src share no bytes.
  * pg_pages_compact: in place; count[0] = number of live pages (live[p] != 0); live pages at or behind count move, in ascending
  * order, to the dead places below it.  map[p] = the new place of old page p, -1 if it was freed.  Contents of pages at or
- * behind count are left as they were.  ws: pg_pages_compact_workspace_bytes. */
+ * behind count are left as they were.  ws: pg_pages_compact_workspace_bytes (0 for few pages: ws may be NULL). */
 PG_API int pg_pages_reorder(const pg_plane* planes, int n_planes, int n_groups, int K, const int32_t* parents, void* stream);
 PG_API int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_planes, int n_dst, int n_src, const int32_t* index,
                          void* stream);

@@ -2,9 +2,26 @@
 #include "pg_host.h"
 #include "../../include/polygon_hip.h"
 
+// What a move kernel needs of a cache: its planes, and where each plane's first column segment is counted.  A segment is
+// PG_SEG bytes of a page: 16 bytes for each lane of a wave.
+constexpr int PG_SEG = 1024;
 struct Planes {
   pg_plane p[PG_MAX_PLANES];
+  int first[PG_MAX_PLANES + 1];
+  int n;
 };
+static int make_planes(const char* who, const pg_plane* planes, int n, Planes* out) {
+  long at = 0;
+  for (int i = 0; i < n; ++i) {
+    out->p[i] = planes[i];
+    out->first[i] = (int)at;
+    at += (planes[i].bytes + PG_SEG - 1) / PG_SEG;
+    PG_REQUIRE(at < (1L << 30), "%s: pages of more than 2^40 bytes", who);
+  }
+  out->first[n] = (int)at;
+  out->n = n;
+  return PG_OK;
+}
 
 // Two planes of `pages` pages share bytes: their spans overlap, unless they interleave with one pitch.
 static bool planes_share(const pg_plane& a, long na, const pg_plane& b, long nb) {
@@ -27,86 +44,216 @@ static int check_planes(const char* who, const pg_plane* planes, int n_planes, l
   return PG_OK;
 }
 
-// In place: a thread owns one byte column of a group's K pages, reads what moves before it writes, so any parents will do.
-__global__ __launch_bounds__(256) void pages_reorder_kernel(Planes pl, int K, const int32_t* __restrict__ parents) {
-  const pg_plane p = pl.p[blockIdx.y];
-  const long g = blockIdx.x;
-  unsigned char* base = (unsigned char*)p.base + g * K * p.pitch;
-  for (long c = threadIdx.x; c < p.bytes; c += blockDim.x) {
-    unsigned char v[PG_MAX_BEAMS];
+// One lane's 16 bytes of a page, `left` >= 1 of them inside it.  Any alignment: the hardware takes unaligned wide accesses.
+__device__ __forceinline__ uint4 page_load(const unsigned char* p, long left) {
+  uint4 v = {0, 0, 0, 0};
+  if (left >= 16) { __builtin_memcpy(&v, p, 16); return v; }
+  int o = 0;
+  if (left & 8) { __builtin_memcpy(&v.x, p, 4); __builtin_memcpy(&v.y, p + 4, 4); o = 8; }
+  if (left & 4) { __builtin_memcpy(&v.z, p + o, 4); o += 4; }
+  if (left & 2) { unsigned short h; __builtin_memcpy(&h, p + o, 2); v.w = h; o += 2; }
+  if (left & 1) v.w |= (unsigned)p[o] << 16;
+  return v;
+}
+__device__ __forceinline__ void page_store(unsigned char* p, long left, const uint4& v) {
+  if (left >= 16) { __builtin_memcpy(p, &v, 16); return; }
+  int o = 0;
+  if (left & 8) { __builtin_memcpy(p, &v.x, 4); __builtin_memcpy(p + 4, &v.y, 4); o = 8; }
+  if (left & 4) { __builtin_memcpy(p + o, &v.z, 4); o += 4; }
+  if (left & 2) { const unsigned short h = (unsigned short)v.w; __builtin_memcpy(p + o, &h, 2); o += 2; }
+  if (left & 1) p[o] = (unsigned char)(v.w >> 16);
+}
+// plane and column of segment `seg` (wave-uniform)
+__device__ __forceinline__ int seg_plane(const Planes& pl, int seg) {
+  int i = 0;
+  while (i + 1 < pl.n && seg >= pl.first[i + 1]) ++i;
+  return i;
+}
+
+// Moves of pages: R pages at a time in one column segment, one wave; every load of a wave is issued before its first store.
+// REORDER: the R pages are a group's K (<= R) and the sources lie among them, so whatever the parents are no page is
+// overwritten before all of the segment's sources are in registers, and no other wave touches this segment of the group.
+// Pages that keep their state are not touched.  Fork: the R pages are consecutive pages of dst, their sources pages of src.
+// Bound by HBM: 16 bytes per lane, up to R loads in flight per wave.
+template <int R, bool REORDER>
+__global__ __launch_bounds__(256) void pages_move_kernel(Planes dst, Planes src, long units, int K, long n_dst, unsigned n_src,
+                                                         const int32_t* __restrict__ from) {
+  const int lane = threadIdx.x & 63;
+  const int segs = dst.first[dst.n];
+  for (long u = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (long)gridDim.x * 4) {
+    const long g = u / segs;
+    const int seg = (int)(u - g * segs), i = seg_plane(dst, seg);
+    const long col = (long)(seg - dst.first[i]) * PG_SEG + lane * 16, left = dst.p[i].bytes - col;
+    const long page0 = g * K, dp = dst.p[i].pitch, sp = REORDER ? dp : src.p[i].pitch;
+    unsigned char* d = (unsigned char*)dst.p[i].base + page0 * dp + col;
+    const unsigned char* s = REORDER ? d : (const unsigned char*)src.p[i].base + col;
+    const int mine = lane < K && page0 + lane < n_dst ? from[page0 + lane] : -1;
+    int f[R];
+    uint4 v[R];
 #pragma unroll
-    for (int j = 0; j < PG_MAX_BEAMS; ++j)
-      if (j < K) {
-        const unsigned from = parents[g * K + j];
-        v[j] = base[(from < (unsigned)K ? from : j) * p.pitch + c];
+    for (int j = 0; j < R; ++j) {
+      f[j] = __builtin_amdgcn_readlane(mine, j);
+      const bool moves = j < K && (unsigned)f[j] < (REORDER ? (unsigned)K : n_src) && !(REORDER && f[j] == j);
+      f[j] = moves ? f[j] : -1;
+      if (f[j] >= 0 && left > 0) v[j] = page_load(s + f[j] * sp, left);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (f[j] >= 0 && left > 0) page_store(d + j * dp, left, v[j]);
+  }
+}
+// waves of 4 per workgroup; more units than this many workgroups hold are taken in rounds
+static int move_grid(long units) { return (int)std::min<long>((units + 3) / 4, 1 << 20); }
+
+// ---- compaction -------------------------------------------------------------------------------------------------------
+// With count live pages, the i-th dead page below count is filled by the i-th live page at or behind it: as few moves as there
+// can be, and no page is both read and written.  before(p) = live pages before p gives every place at once: a dead p < count
+// is hole number p - before(p), a live p >= count is mover number before(p) - before(count).
+
+// the live flags of pages p0 .. p0+7 (those below n) as 8 bits
+__device__ __forceinline__ unsigned live_bits8(const uint8_t* __restrict__ live, long p0, long n) {
+  unsigned long long w = 0;
+  if (p0 + 8 <= n) {
+    __builtin_memcpy(&w, live + p0, 8);
+    w |= w >> 4; w |= w >> 2; w |= w >> 1;
+    w &= 0x0101010101010101ull;
+    return (unsigned)((w * 0x0102040810204080ull) >> 56);   // byte i -> bit i
+  }
+  unsigned m = 0;
+  for (int i = 0; i < 8; ++i)
+    if (p0 + i < n && live[p0 + i]) m |= 1u << i;
+  return m;
+}
+// sum over the workgroup of all threads before this one; *total = over all
+template <int NT> __device__ __forceinline__ int block_before(int x, int* total, int* part) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(s, o);
+    if (lane >= o) s += t;
+  }
+  if (lane == 63) part[wave] = s;
+  __syncthreads();
+  int b = 0, t = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    b += w < wave ? part[w] : 0;
+    t += part[w];
+  }
+  *total = t;
+  return b + s - x;
+}
+// The moves, one wave per MV consecutive column segments: MV loads in flight, then the stores.
+constexpr int MV = 4;
+template <typename I>
+__device__ __forceinline__ void move_pages(const Planes& pl, long moves, const I* hole, const I* mover) {
+  const int lane = threadIdx.x & 63, segs = pl.first[pl.n];
+  const long items = moves * segs;
+  for (long u = ((long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * MV; u < items; u += (long)gridDim.x * 4 * MV) {
+    uint4 v[MV];
+    unsigned char* to[MV];
+    long left[MV];
+    long m = u / segs;
+    int seg = (int)(u - m * segs);
+#pragma unroll
+    for (int j = 0; j < MV; ++j) {
+      left[j] = 0;
+      if (u + j < items) {
+        const int i = seg_plane(pl, seg);
+        const long col = (long)(seg - pl.first[i]) * PG_SEG + lane * 16;
+        left[j] = pl.p[i].bytes - col;
+        const unsigned char* from = (const unsigned char*)pl.p[i].base + mover[m] * pl.p[i].pitch + col;
+        to[j] = (unsigned char*)pl.p[i].base + hole[m] * pl.p[i].pitch + col;
+        if (left[j] > 0) v[j] = page_load(from, left[j]);
+        if (++seg == segs) { seg = 0; ++m; }
       }
+    }
 #pragma unroll
-    for (int j = 0; j < PG_MAX_BEAMS; ++j)
-      if (j < K) base[j * p.pitch + c] = v[j];
+    for (int j = 0; j < MV; ++j)
+      if (left[j] > 0) page_store(to[j], left[j], v[j]);
   }
 }
+static int compact_grid(long n, long segs) { return (int)std::max<long>(1, std::min<long>((n / 2 * segs + 4 * MV - 1) / (4 * MV), 2048)); }
 
-__global__ __launch_bounds__(256) void pages_fork_kernel(Planes dst, Planes src, int n_src, const int32_t* __restrict__ index) {
-  const pg_plane d = dst.p[blockIdx.y], s = src.p[blockIdx.y];
-  const long i = blockIdx.x;
-  const unsigned from = index[i];
-  if (from >= (unsigned)n_src) return;
-  const unsigned char* x = (const unsigned char*)s.base + from * s.pitch;
-  unsigned char* y = (unsigned char*)d.base + i * d.pitch;
-  for (long c = threadIdx.x; c < d.bytes; c += blockDim.x) y[c] = x[c];
-}
-
-// One workgroup: count, then the map and move[i] = the page that goes to the i-th dead place below count, dead[i].
-__global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const uint8_t* __restrict__ live, int32_t* __restrict__ count,
-                                                          int32_t* __restrict__ map, int32_t* __restrict__ dead,
-                                                          int32_t* __restrict__ move) {
-  __shared__ int part[1024];
+// Up to PLAN_PAGES pages: ONE launch, every workgroup works the plan out for itself (n flag bytes from L2, a scan, the moves'
+// ends as 16-bit lists in LDS) and takes its share of the moves.
+constexpr int PLAN_PAGES = 16384;
+__global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, const uint8_t* __restrict__ live,
+                                                            int32_t* __restrict__ count, int32_t* __restrict__ map) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ unsigned long long bits[256];
+  __shared__ int before[256], part[4], low_s;
   const int tid = threadIdx.x;
-  const long per = (n + 1023L) / 1024, p0 = min((long)n, tid * per), p1 = min((long)n, p0 + per);
-  int mine = 0;
-  for (long p = p0; p < p1; ++p) mine += live[p] != 0;
-  part[tid] = mine;
+  const int per = n <= 2048 ? 8 : 64;                       // flags per thread (n <= 256 * per)
+  unsigned long long mine = 0;
+  for (int i = 0; i < per && (long)tid * per + i < n; i += 8) mine |= (unsigned long long)live_bits8(live, (long)tid * per + i, n) << i;
+  int total;
+  const int b = block_before<256>(__popcll(mine), &total, part);
+  bits[tid] = mine;
+  before[tid] = b;
+  // before(count): from the thread that owns page `count`; all of them if that is no page
+  const int end = total - tid * per;                        // my first `end` pages lie below count
+  if (tid == 0 && total == n) low_s = total;
+  if (total < n && end >= 0 && end < per) low_s = b + __popcll(mine & ((1ull << end) - 1));
   __syncthreads();
-  for (int o = 1; o < 1024; o <<= 1) {
-    const int add = tid >= o ? part[tid - o] : 0;
-    __syncthreads();
-    part[tid] += add;
-    __syncthreads();
+  const int low = low_s, moves = total - low;
+  unsigned short *hole = reinterpret_cast<unsigned short*>(smem), *mover = hole + n / 2;
+  const unsigned long long below = end >= 64 ? ~0ull : end > 0 ? (1ull << end) - 1 : 0;
+  const unsigned long long own = n - tid * per >= 64 ? ~0ull : n > tid * per ? (1ull << (n - tid * per)) - 1 : 0;
+  const unsigned long long lane_own = per == 64 ? own : own & 0xFFull;
+  for (unsigned long long h = ~mine & below & lane_own; h; h &= h - 1) {
+    const int i = __ffsll(h) - 1;
+    hole[tid * per + i - (b + __popcll(mine & ((1ull << i) - 1)))] = (unsigned short)(tid * per + i);
   }
-  const int total = part[1023];
-  if (tid == 0) count[0] = total;
-  // live pages before p0, and (for the pages at or behind count) live pages in [count, p0): the moves are as many as the dead
-  // places below count, and the live pages below count are count less that
-  int before = part[tid] - mine;
-  __shared__ int low;
-  if (tid == 0) low = 0;
-  __syncthreads();
-  int below = 0;
-  for (long p = p0; p < p1 && p < total; ++p) below += live[p] != 0;
-  atomicAdd(&low, below);
-  __syncthreads();
-  for (long p = p0; p < p1; ++p) {
-    const bool l = live[p] != 0;
-    if (p < total) {
-      if (!l) dead[p - before] = (int)p;
-      map[p] = l ? (int)p : -1;
-    } else if (l) move[before - low] = (int)p;
-    else map[p] = -1;
-    before += l;
+  for (unsigned long long h = mine & ~below; h; h &= h - 1) {
+    const int i = __ffsll(h) - 1;
+    mover[b + __popcll(mine & ((1ull << i) - 1)) - low] = (unsigned short)(tid * per + i);
   }
   __syncthreads();
-  for (int i = tid; i < total - low; i += 1024) map[move[i]] = dead[i];
+  if (blockIdx.x == 0 && tid == 0) count[0] = total;
+  for (int p = blockIdx.x * 256 + tid; p < n; p += gridDim.x * 256) {
+    const int t = p / per, i = p % per;
+    const bool l = bits[t] >> i & 1;
+    map[p] = !l ? -1 : p < total ? p : (int)hole[before[t] + __popcll(bits[t] & ((1ull << i) - 1)) - low];
+  }
+  move_pages(pl, moves, hole, mover);
 }
-__global__ __launch_bounds__(256) void pages_move_kernel(Planes pl, int n, const int32_t* __restrict__ count,
-                                                         const int32_t* __restrict__ map, const int32_t* __restrict__ move) {
-  const pg_plane p = pl.p[blockIdx.y];
-  const long old = (long)count[0] + blockIdx.x;       // pages at or behind count
-  if (old >= n) return;
-  const int to = map[old];
-  if (to < 0) return;
-  const unsigned char* x = (const unsigned char*)p.base + old * p.pitch;
-  unsigned char* y = (unsigned char*)p.base + to * p.pitch;
-  for (long c = threadIdx.x; c < p.bytes; c += blockDim.x) y[c] = x[c];
+
+// More pages: the plan by one workgroup into the workspace, then the moves.
+__global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const uint8_t* __restrict__ live, int32_t* __restrict__ count,
+                                                          int32_t* __restrict__ map, int32_t* __restrict__ moves,
+                                                          int32_t* __restrict__ hole, int32_t* __restrict__ mover) {
+  __shared__ int part[16], part2[16];
+  const int tid = threadIdx.x;
+  const long per = ((n + 1023L) / 1024 + 7) / 8 * 8, p0 = min((long)n, tid * per), p1 = min((long)n, p0 + per);
+  int mine = 0;
+  for (long p = p0; p < p1; p += 8) mine += __popc(live_bits8(live, p, p1));
+  int total, low;
+  int before = block_before<1024>(mine, &total, part);
+  int under = 0;
+  for (long p = p0; p < p1 && p < total; p += 8) under += __popc(live_bits8(live, p, min(p1, (long)total)));
+  block_before<1024>(under, &low, part2);
+  if (tid == 0) { count[0] = total; moves[0] = total - low; }
+  for (long p = p0; p < p1; p += 8) {
+    const unsigned m = live_bits8(live, p, p1);
+    for (int i = 0; i < 8 && p + i < p1; ++i) {
+      const bool l = m >> i & 1;
+      const long q = p + i;
+      if (q < total) {
+        if (!l) hole[q - before] = (int)q;
+        map[q] = l ? (int)q : -1;
+      } else if (l) mover[before - low] = (int)q;
+      else map[q] = -1;
+      before += l;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < total - low; i += 1024) map[mover[i]] = hole[i];
+}
+__global__ __launch_bounds__(256) void pages_compact_move_kernel(Planes pl, const int32_t* __restrict__ moves,
+                                                                 const int32_t* __restrict__ hole, const int32_t* __restrict__ mover) {
+  move_pages(pl, moves[0], hole, mover);
 }
 
 extern "C" int pg_pages_reorder(const pg_plane* planes, int n_planes, int n_groups, int K, const int32_t* parents, void* stream) {
@@ -116,8 +263,13 @@ extern "C" int pg_pages_reorder(const pg_plane* planes, int n_planes, int n_grou
   if (n_groups == 0) return PG_OK;
   PG_REQUIRE(parents, "pg_pages_reorder: parents is NULL");
   Planes pl;
-  memcpy(pl.p, planes, n_planes * sizeof(pg_plane));
-  hipLaunchKernelGGL(pages_reorder_kernel, dim3(n_groups, n_planes), dim3(256), 0, (hipStream_t)stream, pl, K, parents);
+  PG_TRY(make_planes("pg_pages_reorder", planes, n_planes, &pl));
+  const long units = (long)n_groups * pl.first[n_planes], pages = (long)n_groups * K;
+  const hipStream_t st = (hipStream_t)stream;
+  // R registers of 16 bytes per lane: the narrowest instantiation that holds the group
+  if (K <= 8) hipLaunchKernelGGL((pages_move_kernel<8, true>), dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents);
+  else if (K <= 16) hipLaunchKernelGGL((pages_move_kernel<16, true>), dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents);
+  else hipLaunchKernelGGL((pages_move_kernel<32, true>), dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
@@ -137,30 +289,42 @@ extern "C" int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_pla
   if (n_dst == 0 || n_src == 0) return PG_OK;
   PG_REQUIRE(index, "pg_pages_fork: index is NULL");
   Planes d, s;
-  memcpy(d.p, dst, n_planes * sizeof(pg_plane));
-  memcpy(s.p, src, n_planes * sizeof(pg_plane));
-  hipLaunchKernelGGL(pages_fork_kernel, dim3(n_dst, n_planes), dim3(256), 0, (hipStream_t)stream, d, s, n_src, index);
+  PG_TRY(make_planes("pg_pages_fork", dst, n_planes, &d));
+  PG_TRY(make_planes("pg_pages_fork", src, n_planes, &s));
+  constexpr int R = 8;
+  const long units = (long)cdiv(n_dst, R) * d.first[n_planes];
+  hipLaunchKernelGGL((pages_move_kernel<R, false>), dim3(move_grid(units)), dim3(256), 0, (hipStream_t)stream, d, s, units, R, (long)n_dst,
+                     (unsigned)n_src, index);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
 
-extern "C" size_t pg_pages_compact_workspace_bytes(int n_pages) { return n_pages < 1 ? 256 : align_up((size_t)n_pages * 4, 256) * 2; }
+// number of moves | holes | movers (n / 2 of each at most)
+static size_t compact_list_bytes(int n) { return align_up((size_t)n / 2 * 4 + 4, 256); }
+extern "C" size_t pg_pages_compact_workspace_bytes(int n_pages) {
+  return n_pages <= PLAN_PAGES ? 0 : 256 + 2 * compact_list_bytes(n_pages);
+}
 
 extern "C" int pg_pages_compact(const pg_plane* planes, int n_planes, int n_pages, const uint8_t* live, int32_t* count, int32_t* map,
                                 void* ws, size_t ws_bytes, void* stream) {
   PG_REQUIRE(n_pages >= 0, "pg_pages_compact: n_pages=%d", n_pages);
   PG_TRY(check_planes("pg_pages_compact", planes, n_planes, n_pages));
   PG_REQUIRE(count && (n_pages == 0 || (live && map)), "pg_pages_compact: NULL buffer");
-  if (ws == nullptr || ws_bytes < pg_pages_compact_workspace_bytes(n_pages))
-    PG_FAIL(PG_ERR_WORKSPACE, "pg_pages_compact: workspace too small (%zu < %zu)", ws_bytes, pg_pages_compact_workspace_bytes(n_pages));
+  const size_t need = pg_pages_compact_workspace_bytes(n_pages);
+  if (ws_bytes < need || (need && !ws)) PG_FAIL(PG_ERR_WORKSPACE, "pg_pages_compact: workspace too small (%zu < %zu)", ws_bytes, need);
   Planes pl;
-  memcpy(pl.p, planes, n_planes * sizeof(pg_plane));
-  int32_t *dead = at<int32_t>(ws, 0), *move = at<int32_t>(ws, align_up((size_t)n_pages * 4, 256));
+  PG_TRY(make_planes("pg_pages_compact", planes, n_planes, &pl));
   const hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(1024), 0, st, n_pages, live, count, map, dead, move);
+  const int grid = compact_grid(n_pages, pl.first[n_planes]);
+  if (n_pages <= PLAN_PAGES) {
+    hipLaunchKernelGGL(pages_compact_kernel, dim3(grid), dim3(256), (size_t)(n_pages / 2) * 4, st, pl, n_pages, live, count, map);
+    PG_CHECK_LAUNCH();
+    return PG_OK;
+  }
+  int32_t *moves = at<int32_t>(ws, 0), *hole = at<int32_t>(ws, 256), *mover = at<int32_t>(ws, 256 + compact_list_bytes(n_pages));
+  hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(1024), 0, st, n_pages, live, count, map, moves, hole, mover);
   PG_CHECK_LAUNCH();
-  if (n_pages == 0) return PG_OK;
-  hipLaunchKernelGGL(pages_move_kernel, dim3(n_pages, n_planes), dim3(256), 0, st, pl, n_pages, count, map, move);
+  hipLaunchKernelGGL(pages_compact_move_kernel, dim3(grid), dim3(256), 0, st, pl, moves, hole, mover);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }

@@ -16,10 +16,6 @@ from polygon_amd import _lib
 MAX_BEAMS = 32      # PG_MAX_BEAMS
 
 
-class _Plane(ctypes.Structure):
-    _fields_ = [("base", ctypes.c_void_p), ("pitch", ctypes.c_long), ("bytes", ctypes.c_long)]
-
-
 class BeamStep(NamedTuple):
     """One step of the selection, every member [n, K] and indexed by the place a beam now has."""
     scores: torch.Tensor        # float32: sum of the log-probabilities, -inf where there was no candidate
@@ -47,22 +43,18 @@ def _entries():
     return _entry
 
 
-class _On:
-    """Makes ``device`` the current one for the length of a call (nothing to do where it is) and knows its current stream."""
-
-    def __init__(self, device):
-        if device.type != "cuda":
-            raise _lib.PolygonHipError("polygon_amd computes only on an MI355X (`cuda`) device, got a tensor on %s" % device)
-        self.device, self.before = device, torch.cuda.current_device()
-
-    def __enter__(self):
-        if self.device.index != self.before:
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.device.index != self.before:
-            torch.cuda.set_device(self.before)
+def _call(device, entry, *args):
+    """Runs a C entry on ``device``'s current stream (its last argument), with that device current for the length of the call."""
+    if device.type != "cuda":
+        raise _lib.PolygonHipError("polygon_amd computes only on an MI355X (`cuda`) device, got a tensor on %s" % device)
+    at, now = device.index, torch._C._cuda_getDevice()
+    if at == now:
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(at))
+    else:
+        with torch.cuda.device(at):
+            status = entry(*args, torch._C._cuda_getCurrentRawStream(at))
+    if status != 0:
+        _lib.check(status, entry.__name__)
 
 
 def _flags(t, shape, device, what):
@@ -91,60 +83,63 @@ def beam_select(logits, scores, finished=None, mask=None, temp=1.0, eos=-1, pad=
     if tuple(scores.shape) != (n, K) or scores.dtype != torch.float32 or scores.device != dev:
         raise ValueError("scores must be [%d, %d] float32 on %s, got %s %s on %s" % (n, K, dev, list(scores.shape), scores.dtype,
                                                                                   scores.device))
-    with _On(dev) as stream:
-        L = _entries()
-        if V > 1 and logits.stride(2) != 1:
-            logits = logits.contiguous()
-        scores = scores.contiguous()
-        if finished is not None:
-            finished = _flags(finished, (n, K), dev, "finished")
-        mg = mr = 0
-        if mask is not None:
-            if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev:
-                raise ValueError("mask must be bool or uint8 on %s, got %s on %s" % (dev, mask.dtype, mask.device))
-            if not 1 <= mask.dim() <= 3 or any(a not in (1, b) for a, b in zip(mask.shape[:-1], (n, K)[3 - mask.dim():])) \
-                    or mask.shape[-1] != V:
-                raise ValueError("mask %s does not fit logits %s" % (list(mask.shape), list(logits.shape)))
-            if V > 1 and mask.stride(-1) != 1:
-                mask = mask.contiguous()
-            if mask.dim() > 1 and mask.shape[-2] > 1:
-                mr = mask.stride(-2)
-            if mask.dim() > 2 and mask.shape[0] > 1:
-                mg = mask.stride(0)
-        out = BeamStep(torch.empty(n, K, device=dev), torch.empty(n, K, device=dev, dtype=torch.int32),
-                       torch.empty(n, K, device=dev, dtype=torch.int32), torch.empty(n, K, device=dev, dtype=torch.bool))
-        code = _lib.PG_F32 if logits.dtype == torch.float32 else _lib.PG_BF16
-        need = L.pg_beam_select_workspace_bytes(code, n, K, V)
-        ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
-        _lib.check(L.pg_beam_select(code, logits.data_ptr(), logits.stride(0), logits.stride(1), n, K, V,
-                                    None if mask is None else mask.data_ptr(), mg, mr, float(temp), scores.data_ptr(),
-                                    None if finished is None else finished.data_ptr(), int(eos), int(pad), int(bool(keep_slots)),
-                                    out.scores.data_ptr(), out.parents.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(),
-                                    None if ws is None else ws.data_ptr(), need, stream), "pg_beam_select")
+    if V > 1 and logits.stride(2) != 1:
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    if finished is not None:
+        finished = _flags(finished, (n, K), dev, "finished")
+    mg = mr = 0
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev:
+            raise ValueError("mask must be bool or uint8 on %s, got %s on %s" % (dev, mask.dtype, mask.device))
+        if not 1 <= mask.dim() <= 3 or mask.shape[-1] != V \
+                or any(a not in (1, b) for a, b in zip(mask.shape[:-1], (n, K)[3 - mask.dim():])):
+            raise ValueError("mask %s does not fit logits %s" % (list(mask.shape), list(logits.shape)))
+        if V > 1 and mask.stride(-1) != 1:
+            mask = mask.contiguous()
+        if mask.dim() > 1 and mask.shape[-2] > 1:
+            mr = mask.stride(-2)
+        if mask.dim() > 2 and mask.shape[0] > 1:
+            mg = mask.stride(0)
+    L = _entries()
+    new = scores.new_empty
+    out = BeamStep(new((n, K)), new((n, K), dtype=torch.int32), new((n, K), dtype=torch.int32), new((n, K), dtype=torch.bool))
+    code = _lib.PG_F32 if logits.dtype == torch.float32 else _lib.PG_BF16
+    need = L.pg_beam_select_workspace_bytes(code, n, K, V)
+    ws = new(need, dtype=torch.uint8) if need else None
+    _call(dev, L.pg_beam_select, code, logits.data_ptr(), logits.stride(0), logits.stride(1), n, K, V,
+          None if mask is None else mask.data_ptr(), mg, mr, float(temp), scores.data_ptr(),
+          None if finished is None else finished.data_ptr(), int(eos), int(pad), int(bool(keep_slots)), out.scores.data_ptr(),
+          out.parents.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out
 
 
-def _planes(planes, what, pages=None):
+def _planes(planes, what):
     """The C description of a cache: its planes' first dimension counts pages, what is behind it is one page's dense row."""
     if not planes:
         raise ValueError("%s: no planes" % what)
-    out = (_Plane * len(planes))()
     dev, P = planes[0].device, planes[0].shape[0] if planes[0].dim() else -1
-    for d, t in zip(out, planes):
+    out = []
+    for t in planes:
         if t.dim() < 1 or t.shape[0] != P or t.device != dev:
             raise ValueError("%s: every plane must have the same number of pages in front, on one device" % what)
         if t.requires_grad:
             raise ValueError("%s: pages are moved in place, a plane must not require gradients" % what)
-        row = t.element_size()
-        for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            if size != 1 and stride * t.element_size() != row:
-                raise ValueError("%s: what is behind a plane's first dimension must be dense, got strides %s" % (what, list(t.stride())))
-            row *= size
+        size = t.element_size()
+        if P and t.is_contiguous():
+            row = pitch = t.numel() // P * size
+        else:
+            row, pitch = size, t.stride(0) * size
+            for extent, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+                if extent != 1 and stride * size != row:
+                    raise ValueError("%s: what is behind a plane's first dimension must be dense, got strides %s" % (what, list(t.stride())))
+                row *= extent
+            if P <= 1:
+                pitch = row
         if row == 0:
             raise ValueError("%s: a page of no bytes" % what)
-        d.base, d.bytes = t.data_ptr(), row
-        d.pitch = t.stride(0) * t.element_size() if P > 1 else row
-    return out, dev, P
+        out += (t.data_ptr(), pitch, row)
+    return (ctypes.c_long * len(out))(*out), dev, P
 
 
 def _index(t, dev, what):
@@ -160,9 +155,7 @@ def reorder_pages(planes, parents):
     if parents.dim() != 2 or parents.shape[0] * parents.shape[1] != P:
         raise ValueError("parents %s does not name %d pages" % (list(parents.shape), P))
     parents = _index(parents, dev, "parents")
-    with _On(dev) as stream:
-        _lib.check(_entries().pg_pages_reorder(d, len(planes), parents.shape[0], parents.shape[1], parents.data_ptr(), stream),
-                   "pg_pages_reorder")
+    _call(dev, _entries().pg_pages_reorder, d, len(planes), parents.shape[0], parents.shape[1], parents.data_ptr())
 
 
 def fork_pages(dst, src, index):
@@ -175,8 +168,7 @@ def fork_pages(dst, src, index):
     if tuple(index.shape) != (P,):
         raise ValueError("index %s does not name a page for each of %d" % (list(index.shape), P))
     index = _index(index, dev, "index")
-    with _On(dev) as stream:
-        _lib.check(_entries().pg_pages_fork(d, s, len(dst), P, Q, index.data_ptr(), stream), "pg_pages_fork")
+    _call(dev, _entries().pg_pages_fork, d, s, len(dst), P, Q, index.data_ptr())
 
 
 def compact_pages(planes, live):
@@ -185,12 +177,10 @@ def compact_pages(planes, live):
     page, -1 for a freed one), both on the device."""
     d, dev, P = _planes(planes, "compact_pages")
     live = _flags(live, (P,), dev, "live")
-    with _On(dev) as stream:
-        L = _entries()
-        count = torch.empty(1, device=dev, dtype=torch.int32)
-        where = torch.empty(P, device=dev, dtype=torch.int32)
-        need = L.pg_pages_compact_workspace_bytes(P)
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
-        _lib.check(L.pg_pages_compact(d, len(planes), P, live.data_ptr(), count.data_ptr(), where.data_ptr(), ws.data_ptr(), need,
-                                      stream), "pg_pages_compact")
+    L = _entries()
+    need = L.pg_pages_compact_workspace_bytes(P)
+    count = torch.empty(1, device=dev, dtype=torch.int32)
+    where, ws = count.new_empty(P), count.new_empty(need, dtype=torch.uint8) if need else None
+    _call(dev, L.pg_pages_compact, d, len(planes), P, live.data_ptr(), count.data_ptr(), where.data_ptr(),
+          None if ws is None else ws.data_ptr(), need)
     return count, where
