@@ -1,158 +1,408 @@
 // Beam search: selection over beams and vocabulary.
 #include <math.h>
+#include "pg_beam.h"
 #include "pg_host.h"
-#include "../../include/polygon_hip.h"
 
-struct BeamSelect {
-  const void* logits;
-  long ld_group, ld_row;
-  int n, K, V;
-  const uint8_t* mask;
-  long mask_group, mask_row;
-  double inv_temp;
-  const float* scores;
-  const uint8_t* finished;
-  int eos, pad, keep;
-  float* scores_out;
-  int32_t *parents, *tokens;
-  uint8_t* finished_out;
-};
-
-// The score's bits in the order of the numbers, above the flat index counted down: one 64-bit maximum finds the best score
-// and, among equal ones, the lowest index.  0 = no candidate (c is never NaN or -inf here).
-__device__ __forceinline__ unsigned long long beam_key(float c, unsigned flat) {
-  const unsigned b = __float_as_uint(c);
-  const unsigned o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return ((unsigned long long)o << 32) | (0xFFFFFFFFu - flat);
-}
-__device__ __forceinline__ unsigned beam_key_flat(unsigned long long k) { return 0xFFFFFFFFu - (unsigned)k; }
-__device__ __forceinline__ float beam_key_score(unsigned long long k) {
-  const unsigned o = (unsigned)(k >> 32);
-  return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
-}
-// c of a candidate: the normaliser in 64 bits (which candidate wins hangs on it), rounded to fp32 once, added in fp32.
-// (+ 0.0f: -0.0 and 0.0 are one score and go by the index.)
-__device__ __forceinline__ float beam_score(float x, float m, double inv_temp, double lse, float s) {
-  return (s + (float)(((double)x - (double)m) * inv_temp - lse)) + 0.0f;
-}
-
-// One workgroup per group: every row's maximum and normaliser, then K times the largest key below the last one.
-template <typename T> __global__ __launch_bounds__(256) void beam_select_kernel(BeamSelect a) {
-  __shared__ double red[4];
-  __shared__ unsigned long long redk[4];
-  __shared__ float rm[PG_MAX_BEAMS];
-  __shared__ double rl[PG_MAX_BEAMS];
-  __shared__ int rs[PG_MAX_BEAMS];       // 0 none, 1 alive, 2 finished
-  __shared__ unsigned long long won[PG_MAX_BEAMS];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const long g = blockIdx.x;
+// ---- short vocabularies (V <= 128): one wave per group ---------------------------------------------------------------
+// 16 lanes hold a row (E = 4 or 8 neighbouring symbols per lane, one wide load), 4 rows at a time, P times: the whole group
+// stays in registers (at most 64 of them), so the logits are read once, and all reductions are inside 16 lanes (DPP).
+constexpr int SW = 4;      // waves (groups) per workgroup
+template <typename T, int E, int P>
+__global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a) {
+  __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
+  __shared__ double sum_s[SW][PG_MAX_BEAMS];
+  __shared__ int place_s[SW][PG_MAX_BEAMS];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long g = (long)blockIdx.x * SW + __builtin_amdgcn_readfirstlane(wave);
+  if (g >= a.n) return;                       // no barrier below: waves are on their own
+  const int K = a.K, V = a.V, sub = lane & 15, v0 = sub * E;
+  // beam `lane`
+  float s_mine = -INFINITY;
+  bool fin_mine = false;
+  if (lane < K) {
+    s_mine = a.scores[g * K + lane];
+    fin_mine = a.finished && a.finished[g * K + lane];
+  }
+  const unsigned fin = (unsigned)__ballot(fin_mine), alive = (unsigned)__ballot(isfinite(s_mine)), open = alive & ~fin;
   const T* x0 = (const T*)a.logits + g * a.ld_group;
-  const uint8_t* m0 = a.mask ? a.mask + g * a.mask_group : nullptr;
-  for (int k = 0; k < a.K; ++k) {
-    const float s = a.scores[g * a.K + k];
-    const bool fin = a.finished && a.finished[g * a.K + k];
-    const bool ok = isfinite(s);
+  float x[P][E], m[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int k = p * 4 + (lane >> 4);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[p][e] = -INFINITY;
+    if (!(open >> k & 1) || v0 >= V) continue;
+    const T* r = x0 + k * a.ld_row + v0;
+    const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row + v0 : nullptr;
+    if (v0 + E <= V) {
+      T t[E];
+      __builtin_memcpy(t, r, sizeof(t));
+      uint8_t ok[E];
+      if (mk) __builtin_memcpy(ok, mk, E);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[p][e] = !mk || ok[e] ? to_f32<T>(t[e]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (v0 + e < V && (!mk || mk[e])) x[p][e] = to_f32<T>(r[e]);
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
     float mx = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      bad |= !(x[p][e] < INFINITY);            // NaN or +inf: the row's maximum becomes +inf, and the beam has no continuation
+      mx = fmaxf(mx, x[p][e]);
+    }
+    m[p] = max16(bad ? INFINITY : mx);
     double sum = 0.0;
-    if (ok && !fin) {
-      const T* x = x0 + k * a.ld_row;
-      const uint8_t* mk = m0 ? m0 + k * a.mask_row : nullptr;
-      bool bad = false;
-      for (int v = tid; v < a.V; v += 256) {
-        const float f = to_f32<T>(x[v]);
-        if (mk && !mk[v]) continue;
-        bad |= !(f < INFINITY);
-        mx = fmaxf(mx, f);
-      }
-      if (bad) mx = INFINITY;
-      for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-      if (lane == 0) red[wave] = mx;
-      __syncthreads();
-      mx = fmaxf(fmaxf((float)red[0], (float)red[1]), fmaxf((float)red[2], (float)red[3]));
-      __syncthreads();
-      if (isfinite(mx)) {
-        for (int v = tid; v < a.V; v += 256)
-          if (!mk || mk[v]) sum += exp(((double)to_f32<T>(x[v]) - (double)mx) * a.inv_temp);
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-        if (lane == 0) red[wave] = sum;
-        __syncthreads();
-        sum = (red[0] + red[1]) + (red[2] + red[3]);
-        __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += beam_exp(((double)x[p][e] - (double)m[p]) * a.inv_temp);
+    sum = sum16(sum);
+    if (sub == 0) sum_s[wave][p * 4 + (lane >> 4)] = sum;
+  }
+  wave_sync();
+  // one logarithm for all rows
+  if (lane < P * 4) sum_s[wave][lane] = log(sum_s[wave][lane]);
+  wave_sync();
+  unsigned order[P * E];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int k = p * 4 + (lane >> 4);
+    const float s = __shfl(s_mine, k);
+    const double lse = sum_s[wave][k];
+    const bool has = (open >> k & 1) && isfinite(m[p]), done = alive & fin & (1u << k);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float c = has ? beam_score(x[p][e], m[p], a.inv_temp, lse, s) : -INFINITY;
+      if (done && v0 + e == a.pad) c = s + 0.0f;
+      order[p * E + e] = c > -INFINITY ? beam_order(c) : 0;
+    }
+  }
+  beam_best<P * E>(order, [&](int i) { return (unsigned)((i / E * 4 + (lane >> 4)) * V + v0 + i % E); }, 0, K, list_s[wave],
+                   won_s[wave], lane);
+  beam_write(a, g, won_s[wave], fin, place_s[wave], lane);
+}
+
+// ---- long vocabularies ------------------------------------------------------------------------------------------------
+// The vocabulary is split into chunks; a wave walks through its chunk in tiles of 64 x 16 symbols held in registers, with a
+// running maximum and 64-bit sum of the softmax and the K best logits so far (a tile's symbols at or below the K-th best are
+// out at one comparison per lane).  A chunk leaves (max, sum, K keys of logit and symbol).  A workgroup per group then joins
+// the chunks' sums, turns their keys into scores and selects.
+constexpr int LE = 16, TILE = 64 * LE;
+struct BeamChunk {
+  double sum;
+  float max;       // +inf: a NaN or +inf was seen
+  int pad;
+};
+struct BeamLong {
+  int chunks, tiles;             // per row; tiles per chunk
+  BeamChunk* part;               // [n * K, chunks]
+  unsigned long long* keys;      // [n * K, chunks, K]
+};
+template <typename T>
+__global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamLong l) {
+  __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long u = (long)blockIdx.x * SW + __builtin_amdgcn_readfirstlane(wave);
+  const long row = u / l.chunks;
+  const int chunk = (int)(u - row * l.chunks), K = a.K, V = a.V;
+  if (row >= (long)a.n * K) return;
+  if (!isfinite(a.scores[row]) || (a.finished && a.finished[row])) return;     // the join does not look at this row
+  const long g = row / K;
+  const int k = (int)(row - g * K);
+  const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row;
+  const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row : nullptr;
+  float mx = -INFINITY;
+  double sum = 0.0;
+  bool bad = false;
+  unsigned above = 0;            // order of the K-th best so far (0: fewer than K)
+  unsigned long long mine = 0;   // lane j: the j-th best key so far
+  for (int t = 0; t < l.tiles; ++t) {
+    const long b = ((long)chunk * l.tiles + t) * TILE;
+    if (b >= V) break;
+    float x[LE];
+    // 16-byte loads: 4 (fp32) or 8 (bf16) neighbouring symbols per lane and load, a wave's loads dense
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int q = 0; q < LE / W; ++q) {
+      const long v = b + (q * 64 + lane) * W;
+      if (v + W <= V) {
+        T e[W];
+        __builtin_memcpy(e, r + v, sizeof(e));
+        uint8_t ok[W];
+        if (mk) __builtin_memcpy(ok, mk + v, W);
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[q * W + i] = !mk || ok[i] ? to_f32<T>(e[i]) : -INFINITY;
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[q * W + i] = v + i < V && (!mk || mk[v + i]) ? to_f32<T>(r[v + i]) : -INFINITY;
       }
     }
-    if (tid == 0) {
-      rs[k] = !ok ? 0 : fin ? 2 : isfinite(mx) ? 1 : 0;
-      rm[k] = mx;
-      rl[k] = log(sum);
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < LE; ++i) {
+      bad |= !(x[i] < INFINITY);
+      top = fmaxf(top, x[i]);
+    }
+    const float all = max64(top);
+    if (!(all > -INFINITY) || all == INFINITY) continue;
+    if (all > mx) {
+      sum *= beam_exp(((double)mx - (double)all) * a.inv_temp);
+      mx = all;
+    }
+#pragma unroll
+    for (int i = 0; i < LE; ++i) sum += beam_exp(((double)x[i] - (double)mx) * a.inv_temp);
+    if (!__ballot(top > -INFINITY && beam_order(top) > above)) continue;
+    unsigned order[LE];
+#pragma unroll
+    for (int i = 0; i < LE; ++i) order[i] = x[i] > -INFINITY ? beam_order(x[i]) : 0;
+    beam_best<LE>(order, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, above, K, list_s[wave], won_s[wave],
+                  lane);
+    if (t == 0) mine = lane < K ? won_s[wave][lane] : 0;
+    else {   // the K best of two lists of K
+      if (lane < K) list_s[wave][lane] = won_s[wave][lane];
+      const unsigned long long old = __ballot(mine != 0), fresh = __ballot(lane < K && won_s[wave][lane] != 0);
+      const int nf = __popcll(fresh);
+      if (mine) list_s[wave][nf + lanes_before(old)] = mine;
+      wave_sync();
+      beam_rank(list_s[wave], nf + __popcll(old), won_s[wave], K, lane);
+      mine = lane < K ? won_s[wave][lane] : 0;
+    }
+    above = __builtin_amdgcn_readlane((int)(mine >> 32), K - 1);
+  }
+  const bool any_bad = __ballot(bad) != 0;
+  sum = sum64(sum);
+  if (lane == 0) l.part[row * l.chunks + chunk] = {sum, any_bad ? INFINITY : mx, 0};
+  if (lane < K) l.keys[(row * l.chunks + chunk) * K + lane] = mine;
+}
+
+constexpr int JW = 4, JLIST = 1024;
+template <typename T>
+__global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLong l) {
+  __shared__ unsigned long long list[JLIST], won[PG_MAX_BEAMS], red[JW];
+  __shared__ double lse_s[PG_MAX_BEAMS];
+  __shared__ float max_s[PG_MAX_BEAMS], score_s[PG_MAX_BEAMS];
+  __shared__ int place[PG_MAX_BEAMS], again[64 * JW], have, stop;
+  __shared__ unsigned best_s[64 * JW];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, K = a.K, V = a.V;
+  const long g = blockIdx.x;
+  float s_mine = -INFINITY;
+  bool fin_mine = false;
+  if (lane < K) {
+    s_mine = a.scores[g * K + lane];
+    fin_mine = a.finished && a.finished[g * K + lane];
+  }
+  const unsigned fin = (unsigned)__ballot(fin_mine), alive = (unsigned)__ballot(isfinite(s_mine)), open = alive & ~fin;
+  if (wave == 0 && lane < K) score_s[lane] = s_mine;
+  // every row's maximum and normaliser from its chunks
+  for (int k = wave; k < K; k += JW) {
+    float mx = -INFINITY;
+    double sum = 0.0;
+    if (open >> k & 1) {
+      const BeamChunk* part = l.part + (g * K + k) * l.chunks;
+      for (int c = lane; c < l.chunks; c += 64) mx = fmaxf(mx, part[c].max);
+      mx = max64(mx);
+      if (isfinite(mx))
+        for (int c = lane; c < l.chunks; c += 64) sum += part[c].sum * beam_exp(((double)part[c].max - (double)mx) * a.inv_temp);
+      sum = sum64(sum);
+    }
+    if (lane == 0) { max_s[k] = mx; lse_s[k] = log(sum); }
+  }
+  if (tid == 0) have = 0;
+  __syncthreads();
+  // an entry's score, or 0: entry e of the group's K * chunks * K
+  const int per_row = l.chunks * K, total = K * per_row;
+  const unsigned long long* keys = l.keys + g * (long)total;
+  auto entry = [&](int e) -> unsigned long long {
+    const int k = e / per_row;
+    if (!(open >> k & 1) || !isfinite(max_s[k])) return 0;
+    const unsigned long long key = keys[e];
+    if (!key) return 0;
+    const float c = beam_score(beam_key_number(key), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
+    return c > -INFINITY ? beam_key(beam_order(c), (unsigned)(k * V) + beam_key_index(key)) : 0;
+  };
+  auto ended = [&](int k) -> unsigned long long {      // a finished beam's own candidate
+    return alive & fin & (1u << k) ? beam_key(beam_order(score_s[k] + 0.0f), (unsigned)(k * V + a.pad)) : 0;
+  };
+  // a bound that at least K of the threads' bests reach (found in every wave alike)
+  unsigned best = tid < K ? (unsigned)(ended(tid) >> 32) : 0;
+  for (int e = tid; e < total; e += 64 * JW) best = max(best, (unsigned)(entry(e) >> 32));
+  best_s[tid] = best;
+  __syncthreads();
+  unsigned b4[JW], bound = 1;
+#pragma unroll
+  for (int w = 0; w < JW; ++w) b4[w] = best_s[w * 64 + lane];
+  {
+    int some = 0;
+    unsigned lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+    for (int w = 0; w < JW; ++w) {
+      some += __popcll(__ballot(b4[w] != 0));
+      if (b4[w]) lo = min(lo, b4[w]);
+      hi = max(hi, b4[w]);
+    }
+    for (int o = 32; o; o >>= 1) {
+      lo = min(lo, (unsigned)__shfl_xor(lo, o));
+      hi = max(hi, (unsigned)__shfl_xor(hi, o));
+    }
+    if (some > K) {
+      hi += 1;
+      while (hi - lo > 1) {
+        const unsigned mid = lo + (hi - lo) / 2;
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < JW; ++w) c += __popcll(__ballot(b4[w] >= mid));
+        if (c >= K) {
+          lo = mid;
+          if (c <= K + 4 + K / 4) break;
+        } else hi = mid;
+      }
+      bound = lo;
+    }
+  }
+  auto put = [&](unsigned long long key) {
+    if ((unsigned)(key >> 32) < bound) return;
+    const int at = atomicAdd(&have, 1);       // the list's order does not matter: its keys are ranked
+    if (at < JLIST) list[at] = key;
+  };
+  if (tid < K) put(ended(tid));
+  for (int e = tid; e < total; e += 64 * JW) put(entry(e));
+  if (tid < K) won[tid] = 0;
+  __syncthreads();
+  const int m = have;
+  if (m <= JLIST) {
+    for (int i = tid; i < m; i += 64 * JW) {
+      const unsigned long long key = list[i];
+      int r = 0;
+      for (int j = 0; j < m; ++j) r += list[j] > key;
+      if (r < K) won[r] = key;
+    }
+  } else {   // ties all over: the keys one by one
+    unsigned long long last = ~0ull;
+    for (int j = 0; j < K; ++j) {
+      unsigned long long top = 0;
+      auto see = [&](unsigned long long key) { if (key < last && key > top) top = key; };
+      if (tid < K) see(ended(tid));
+      for (int e = tid; e < total; e += 64 * JW) see(entry(e));
+      top = max64(top);
+      if (lane == 0) red[wave] = top;
+      __syncthreads();
+      for (int w = 0; w < JW; ++w) top = red[w] > top ? red[w] : top;
+      last = top;
+      if (tid == 0) won[j] = top;
+      __syncthreads();
     }
   }
   __syncthreads();
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < a.K; ++j) {
-    unsigned long long best = 0;
-    if (last)
-      for (int k = 0; k < a.K; ++k) {
-        const float s = a.scores[g * a.K + k];
-        if (rs[k] == 2 && tid == 0) {
-          const unsigned long long key = beam_key(s + 0.0f, k * a.V + a.pad);
-          if (key < last && key > best) best = key;
-        }
-        if (rs[k] != 1) continue;
-        const T* x = x0 + k * a.ld_row;
-        const uint8_t* mk = m0 ? m0 + k * a.mask_row : nullptr;
-        for (int v = tid; v < a.V; v += 256) {
+  // A chunk's list goes by the logit, the selection by the score, and rounding can give symbols with different logits one
+  // score: then the lower index counts.  What a full list left out can only matter if the list's last entry has exactly the
+  // score of the group's last winner (a better one would make K + 1 winners); such a chunk is read again for the symbols of
+  // that score.  It takes all of a group's winners coming from one chunk.
+  const unsigned edge = (unsigned)(won[K - 1] >> 32);
+  if (edge == 0) {
+    if (wave == 0) beam_write(a, g, won, fin, place, lane);
+    return;
+  }
+  for (int base = 0; base < K * l.chunks; base += 64 * JW) {
+    if (tid == 0) have = 0;
+    __syncthreads();
+    {
+      const int kc = base + tid;       // (beam, chunk); one that starts behind the last winner cannot hold a lower index
+      if (kc < K * l.chunks && (unsigned)(entry(kc * K + K - 1) >> 32) == edge &&
+          (unsigned)(kc / l.chunks * V) + (unsigned)(kc % l.chunks) * l.tiles * TILE < beam_key_index(won[K - 1]))
+        again[atomicAdd(&have, 1)] = kc;
+    }
+    __syncthreads();
+    const int again_n = have;
+    for (int i = 0; i < again_n; ++i) {
+      const int k = again[i] / l.chunks, c = again[i] % l.chunks;
+      const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row;
+      const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row : nullptr;
+      const long v1 = min((long)V, (long)(c + 1) * l.tiles * TILE);
+      // the symbols of the edge's score, lowest first, until one does not beat the last winner
+      unsigned long long last = ~0ull;
+      for (int round = 0; round < K; ++round) {
+        unsigned long long top = 0;
+        for (long v = (long)c * l.tiles * TILE + tid; v < v1; v += 64 * JW) {
           if (mk && !mk[v]) continue;
-          const float c = beam_score(to_f32<T>(x[v]), rm[k], a.inv_temp, rl[k], s);
-          if (!(c > -INFINITY)) continue;
-          const unsigned long long key = beam_key(c, k * a.V + v);
-          if (key < last && key > best) best = key;
+          const float sc = beam_score(to_f32<T>(r[v]), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
+          if (!(sc > -INFINITY) || beam_order(sc) != edge) continue;
+          const unsigned long long key = beam_key(edge, (unsigned)(k * V + v));
+          if (key < last && key > top) top = key;
         }
+        top = max64(top);
+        if (lane == 0) red[wave] = top;
+        __syncthreads();
+        for (int w = 0; w < JW; ++w) top = red[w] > top ? red[w] : top;
+        last = top;
+        if (tid == 0) {      // into the winners, if it beats the last one and is not there yet
+          bool in = top > won[K - 1];
+          for (int j = 0; j < K; ++j) in &= won[j] != top;
+          if (in) {
+            int j = K - 1;
+            for (; j > 0 && won[j - 1] < top; --j) won[j] = won[j - 1];
+            won[j] = top;
+          }
+          stop = top == 0 || top < won[K - 1];
+        }
+        __syncthreads();
+        if (stop) break;
       }
-    for (int o = 32; o; o >>= 1) {
-      const unsigned long long other = __shfl_xor(best, o);
-      best = other > best ? other : best;
+      __syncthreads();
     }
-    if (lane == 0) redk[wave] = best;
-    __syncthreads();
-    best = redk[0];
-    for (int w = 1; w < 4; ++w) best = redk[w] > best ? redk[w] : best;
-    last = best;
-    if (tid == 0) won[j] = best;
     __syncthreads();
   }
-  if (tid != 0) return;
-  // read every flag before any is written: the outputs may be the inputs
-  unsigned fin = 0, taken = 0;
-  for (int k = 0; k < a.K; ++k) fin |= (unsigned)(rs[k] == 2) << k;
-  int place[PG_MAX_BEAMS];
-  for (int j = 0; j < a.K; ++j) {
-    place[j] = j;
-    if (!a.keep) continue;
-    const int p = won[j] ? (int)(beam_key_flat(won[j]) / a.V) : -1;
-    place[j] = -1;
-    if (p >= 0 && !(taken >> p & 1)) { place[j] = p; taken |= 1u << p; }
-  }
-  for (int j = 0; j < a.K; ++j) {
-    int p = place[j];
-    if (p < 0) { p = __ffs(~taken) - 1; taken |= 1u << p; }
-    const long o = g * a.K + p;
-    if (won[j]) {
-      const unsigned flat = beam_key_flat(won[j]);
-      const int parent = flat / a.V, v = flat % a.V;
-      a.scores_out[o] = beam_key_score(won[j]);
-      a.parents[o] = parent;
-      a.tokens[o] = v;
-      a.finished_out[o] = (fin >> parent & 1) || v == a.eos;
-    } else {
-      a.scores_out[o] = -INFINITY;
-      a.parents[o] = p;
-      a.tokens[o] = a.pad;
-      a.finished_out[o] = 1;
-    }
-  }
+  if (wave == 0) beam_write(a, g, won, fin, place, lane);
 }
 
-extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V) { return 0; }
+constexpr int SHORT_V = 128;
+// Tiles per chunk: as long as there are waves enough for the card (8 on each of its 1024 SIMDs) a chunk is made longer - the
+// K best so far make the next tile cheap, and there are fewer lists to join.
+static BeamLong long_plan(int n, int K, int V) {
+  BeamLong l = {};
+  const long tiles = (V + TILE - 1) / TILE, rows = (long)n * K;
+  l.tiles = (int)std::max<long>(1, std::min<long>(tiles, rows * tiles / 8192));
+  l.chunks = (int)((tiles + l.tiles - 1) / l.tiles);
+  return l;
+}
+
+extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V) {
+  (void)dtype;
+  if (n < 1 || K < 1 || V <= SHORT_V) return 0;
+  const BeamLong l = long_plan(n, K, V);
+  const size_t lists = (size_t)n * K * l.chunks;
+  return align_up(lists * sizeof(BeamChunk), 256) + lists * K * 8;
+}
+
+template <typename T> static int beam_select_t(const BeamSelect& a, void* ws, size_t ws_bytes, hipStream_t st) {
+  if (a.V <= SHORT_V) {
+    const dim3 grid(cdiv(a.n, SW)), block(64 * SW);
+#define PG_SHORT(E, P) hipLaunchKernelGGL((beam_select_short_kernel<T, E, P>), grid, block, 0, st, a)
+#define PG_SHORT_E(E) \
+  do { if (a.K <= 4) PG_SHORT(E, 1); else if (a.K <= 8) PG_SHORT(E, 2); else if (a.K <= 16) PG_SHORT(E, 4); else PG_SHORT(E, 8); } while (0)
+    if (a.V <= 64) PG_SHORT_E(4);
+    else PG_SHORT_E(8);
+#undef PG_SHORT_E
+#undef PG_SHORT
+    PG_CHECK_LAUNCH();
+    return PG_OK;
+  }
+  const size_t need = pg_beam_select_workspace_bytes(0, a.n, a.K, a.V);
+  if (!ws || ws_bytes < need) PG_FAIL(PG_ERR_WORKSPACE, "pg_beam_select: workspace too small (%zu < %zu)", ws_bytes, need);
+  BeamLong l = long_plan(a.n, a.K, a.V);
+  const long lists = (long)a.n * a.K * l.chunks;
+  PG_REQUIRE(lists < (1L << 26), "pg_beam_select: n=%d, K=%d, V=%d are too many rows for one call", a.n, a.K, a.V);
+  l.part = at<BeamChunk>(ws, 0);
+  l.keys = at<unsigned long long>(ws, align_up((size_t)lists * sizeof(BeamChunk), 256));
+  hipLaunchKernelGGL(beam_chunk_kernel<T>, dim3(cdiv(lists, SW)), dim3(64 * SW), 0, st, a, l);
+  PG_CHECK_LAUNCH();
+  hipLaunchKernelGGL(beam_join_kernel<T>, dim3(a.n), dim3(64 * JW), 0, st, a, l);
+  PG_CHECK_LAUNCH();
+  return PG_OK;
+}
 
 extern "C" int pg_beam_select(int dtype, const void* logits, long ld_group, long ld_row, int n, int K, int V,
                               const uint8_t* mask, long mask_group, long mask_row, double temp, const float* scores,
@@ -163,13 +413,11 @@ extern "C" int pg_beam_select(int dtype, const void* logits, long ld_group, long
              "pg_beam_select: n=%d, K=%d outside [1,%d] or V=%d outside [1,%d]", n, K, PG_MAX_BEAMS, V, PG_MAX_BEAM_V);
   PG_REQUIRE(temp > 0.0 && isfinite(temp) && isfinite(1.0 / temp), "pg_beam_select: temperature must be positive and finite");
   PG_REQUIRE(pad >= 0 && pad < V && eos < V, "pg_beam_select: pad=%d outside [0,%d) or eos=%d not below it", pad, V, eos);
+  PG_REQUIRE((long)n * K <= 1L << 26, "pg_beam_select: n * K = %ld above 2^26", (long)n * K);
   if (n == 0) return PG_OK;
   PG_REQUIRE(logits && scores && scores_out && parents && tokens && finished_out, "pg_beam_select: NULL buffer");
-  BeamSelect a = {logits, ld_group, ld_row, n, K, V, mask, mask_group, mask_row, 1.0 / temp, scores, finished, eos, pad, keep_slots,
-                  scores_out, parents, tokens, finished_out};
-  const hipStream_t st = (hipStream_t)stream;
-  if (dtype == PG_BF16) hipLaunchKernelGGL(beam_select_kernel<bf16_t>, dim3(n), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(beam_select_kernel<float>, dim3(n), dim3(256), 0, st, a);
-  PG_CHECK_LAUNCH();
-  return PG_OK;
+  const BeamSelect a = {logits, ld_group, ld_row, n, K, V, mask, mask_group, mask_row, 1.0 / temp, scores, finished, eos, pad, keep_slots,
+                        scores_out, parents, tokens, finished_out};
+  return dtype == PG_BF16 ? beam_select_t<bf16_t>(a, ws, ws_bytes, (hipStream_t)stream)
+                          : beam_select_t<float>(a, ws, ws_bytes, (hipStream_t)stream);
 }

@@ -144,6 +144,27 @@ def test_select_ties_go_to_the_lowest_index(V):
         check_select(flat, -0.0 * scores)
 
 
+@pytest.mark.parametrize("V", [64, 128, 900, 3000, 20000])
+def test_select_ties_made_by_rounding(V):
+    """Logits that differ by less than the score's rounding: one score, so the lower index wins, not the larger logit"""
+    K = 8
+    up = 1.0 + torch.arange(V, device="cuda") * 2.0 ** -23        # the largest logits last
+    logits = up.expand(6, K, V).contiguous()
+    scores = torch.full((6, K), -1000.0, device="cuda")
+    scores[1, 1:] = -INF                                           # one beam holds all winners
+    scores[2, 3] = -900.0
+    scores[3, 5], scores[3, 2] = -900.0, -901.0
+    logits[4] = logits[4].flip(-1)
+    logits[5, :, V // 3: V // 2] += 1e-4                           # part of them above the others' score
+    for keep in (False, True):
+        check_select(logits, scores, keep_slots=keep)
+    got = check_select(logits[:1, :1].contiguous(), scores[:1, :1])   # K = 1: the argmax of the rounded scores
+    assert got.tokens.item() == int(np.argmax(np.float32(-1000.0) + torch.log_softmax(up.double(), 0).float().cpu().numpy()))
+    mask = torch.ones(V, device="cuda", dtype=torch.bool)
+    mask[:5] = False
+    check_select(logits, scores, mask=mask)
+
+
 def test_select_strides():
     logits, scores, fin = make(6, 5, 51, seed=3)
     wide = torch.full((6, 7, 80), float("nan"), device="cuda")
