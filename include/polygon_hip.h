@@ -204,7 +204,7 @@ PG_API int pg_sample_forced(const pg_dims* d, int dtype, const float* params, co
  * read by another is never itself overwritten.
  * logits: dtype, element (g, k, v) at g * ld_group + k * ld_row + v.  mask (nullable): bytes, 0 = forbidden, element (g, k, v)
  * at g * mask_group + k * mask_row + v (0 strides share one mask).  scores_out / finished_out may be scores / finished.
- * K <= PG_MAX_BEAMS, V <= PG_MAX_BEAM_V, n * K <= 2^26.  ws: pg_beam_select_workspace_bytes (0 for short vocabularies: ws may be NULL). */
+ * K <= PG_MAX_BEAMS, V <= PG_MAX_BEAM_V, n * K < 2^24.  ws: pg_beam_select_workspace_bytes (0 for short vocabularies: ws may be NULL). */
 #define PG_MAX_BEAMS 32
 #define PG_MAX_BEAM_V (1 << 20)
 PG_API size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V);

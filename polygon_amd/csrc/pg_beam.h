@@ -9,7 +9,7 @@ struct BeamSelect {
   int n, K, V;
   const uint8_t* mask;
   long mask_group, mask_row;
-  double inv_temp;
+  double inv_temp, scale;            // 1 / temp, log2(e) / temp
   const float* scores;
   const uint8_t* finished;
   int eos, pad, keep;
@@ -22,43 +22,61 @@ struct BeamSelect {
 // A number's bits in the order of the numbers; 0 stands for "nothing" (no number maps to 0).
 __device__ __forceinline__ unsigned beam_order(float c) {
   const unsigned b = __float_as_uint(c);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float beam_unorder(unsigned o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o); }
 // The order above the index counted down: one 64-bit maximum finds the best number and, among equal ones, the lowest index.
-__device__ __forceinline__ unsigned long long beam_key(unsigned order, unsigned index) {
-  return ((unsigned long long)order << 32) | (0xFFFFFFFFu - index);
+// A candidate's index is beam << 20 | symbol, which orders as beam * V + symbol does.  (+ 0.0f: -0.0 and 0.0 are one number.)
+__device__ __forceinline__ unsigned long long beam_key(float c, unsigned index) {
+  return ((unsigned long long)beam_order(c + 0.0f) << 32) | (0xFFFFFFFFu - index);
 }
 __device__ __forceinline__ unsigned beam_key_index(unsigned long long k) { return 0xFFFFFFFFu - (unsigned)k; }
 __device__ __forceinline__ float beam_key_number(unsigned long long k) { return beam_unorder((unsigned)(k >> 32)); }
 
 // ---- exact scores -----------------------------------------------------------------------------------------------------
-// exp of d <= 0 in 64 bits: d = n ln 2 + r with |r| <= ln 2 / 2, the series of exp(r) to r^11 (remainder r^12 / 12! < 7e-15),
-// times 2^n.  18 instructions where the library's, which serves every argument, takes about twice that.  Which candidate wins
-// hangs on the normaliser, so 32 bits are not enough; 7e-15 is far below what a score's rounding to fp32 can tell.
-__device__ __forceinline__ double beam_exp(double d) {
-  d = fmax(d, -800.0);                       // -inf and all that underflows: 0
-  const double n = rint(d * 1.4426950408889634074);
-  double r = fma(n, -6.93147180369123816490e-01, d);   // ln 2 in two parts
-  r = fma(n, -1.90821492927058770002e-10, r);
-  double p = 1.0 / 39916800.0;
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return ldexp(p, (int)n);
+// 2^t of t <= 0 in 64 bits: t = n + f with |f| <= 1/2 (adding 1.5 * 2^52 leaves n in the low bits), 2^f = 1 + f q(f) with q fitted
+// to the least largest relative error of 2^f on that interval, 8.1e-13 (Lawson's iteration), n added to the exponent.  13
+// instructions, all at the full 64-bit rate, which is also that of fp32 here.  Which candidate wins hangs on the normaliser:
+// 32 bits (6e-8) would let near ties flip, 8e-13 is a millionth of what a score's rounding to fp32 can tell.  2^0 is exactly 1.
+constexpr double BEAM_LOG2E = 1.4426950408889634074;
+__device__ __forceinline__ double beam_exp2(double t) {
+  t = fmax(t, -1000.0);                      // -inf and all that would underflow: 1e-301
+  const double big = t + 6755399441055744.0, f = t - (big - 6755399441055744.0);
+  double p = 1.3178933133195561237e-6;
+  p = fma(p, f, 1.5309156473849579456e-5);
+  p = fma(p, f, 1.5403825466894596854e-4);
+  p = fma(p, f, 1.3333454859215948937e-3);
+  p = fma(p, f, 9.618128616111247785e-3);
+  p = fma(p, f, 5.550410935267969742e-2);
+  p = fma(p, f, 2.4022650698110698366e-1);
+  p = fma(p, f, 6.9314718054821182051e-1);
+  p = fma(p, f, 1.0);
+  const long long b = __double_as_longlong(p);
+  const unsigned hi = (unsigned)(b >> 32) + ((unsigned)__double_as_longlong(big) << 20);
+  return __longlong_as_double(((long long)hi << 32) | (unsigned)b);
+}
+// ln of a softmax's sum, 1 <= z <= 2^20: the hardware's log2 (a few 1e-7 off) corrected once by what z falls short of its power,
+// ln z = y ln 2 + ln(z 2^-y), the last factor within 1e-6 of 1.  As exact as beam_exp2; ln 1 is exactly 0.
+__device__ __forceinline__ double beam_log(double z) {
+  const double y = (double)__builtin_amdgcn_logf((float)z), r = fma(z, beam_exp2(-y), -1.0);
+  return fma(y, 0.69314718055994530942, fma(-0.5 * r, r, r));
+}
+// the larger of three; NaN if one is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// a lane's largest number; NaN if it holds one
+template <int N> __device__ __forceinline__ float max_nan(const float (&x)[N]) {
+  float m = N % 2 ? x[0] : max3_nan(x[0], x[N - 1], x[N - 1]);
+#pragma unroll
+  for (int i = 1; i + 1 < N; i += 2) m = max3_nan(m, x[i], x[i + 1]);
+  return m;
 }
 // c of a candidate: the log-probability in 64 bits, rounded to fp32 once, added to the beam's score in fp32.
-// (+ 0.0f: -0.0 and 0.0 are one score and go by the index.)
 __device__ __forceinline__ float beam_score(float x, float m, double inv_temp, double lse, float s) {
-  return (s + (float)(((double)x - (double)m) * inv_temp - lse)) + 0.0f;
+  return s + (float)(((double)x - (double)m) * inv_temp - lse);
 }
 
 // ---- reductions over 16 lanes (every lane gets the result; partners add the same two numbers, so all results are equal) ----
@@ -117,69 +135,92 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 // ---- the K best of a wave's registers --------------------------------------------------------------------------------
-// With one order per lane (each lane's best): a bound such that at least K lanes reach it, and few more - found by halving the
-// interval of orders, where a step costs a comparison and a population count.  1 (everything) if fewer than K lanes have any.
-// Any K of what reaches the bound are at least as good as it, so nothing below the bound can be among the K best.
-__device__ __forceinline__ unsigned beam_bound(unsigned best, int K) {
-  if (__popcll(__ballot(best != 0)) <= K) return 1;
-  unsigned lo = best ? best : 0xFFFFFFFFu, hi = best;
-  for (int o = 32; o; o >>= 1) {
-    lo = min(lo, (unsigned)__shfl_xor(lo, o));
-    hi = max(hi, (unsigned)__shfl_xor(hi, o));
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  hi = __builtin_amdgcn_readfirstlane(hi) + 1;        // (+inf is never an order here: no wrap)
+// With one number per lane (each lane's best; `some` > K lanes exceed `above`): a bound such that at least K lanes reach it,
+// and few more - from the wave's best downwards in doubling strides, then by halving; a step costs one comparison and a
+// population count.  Any K of what reaches the bound are at least as good as it, so nothing below it can be among the K best.
+__device__ __forceinline__ float beam_bound(float best, float above, int K) {
+  const unsigned mine = beam_order(best), none = beam_order(above);      // (never +inf: the sum below cannot wrap)
+  unsigned hi = beam_order(max64(best)) + 1, lo, step = 1u << 20;        // an eighth of an octave to begin with
   const int enough = K + 4 + K / 4;
+  for (;;) {
+    lo = hi - none > step ? hi - step : none + 1;
+    const int c = __popcll(__ballot(mine >= lo));
+    if (c >= K) {
+      if (c <= enough) return beam_unorder(lo);
+      break;
+    }
+    hi = lo;
+    step <<= 1;
+  }
   while (hi - lo > 1) {
     const unsigned mid = lo + (hi - lo) / 2;
-    const int c = __popcll(__ballot(best >= mid));
+    const int c = __popcll(__ballot(mine >= mid));
     if (c >= K) {
       lo = mid;
       if (c <= enough) break;
     } else hi = mid;
   }
-  return lo;
+  return beam_unorder(lo);
 }
 
-// Ranks `m` <= 128 different keys of list[] and puts the `keep` best into won[] in order (won[] beyond m: 0).
-__device__ __forceinline__ void beam_rank(const unsigned long long* list, int m, unsigned long long* won, int keep, int lane) {
-  if (lane < keep) won[lane] = 0;
-  const unsigned long long a = lane < m ? list[lane] : 0, b = lane + 64 < m ? list[lane + 64] : 0;
-  int ra = 0, rb = 0;
+// Ranks `m` <= 128 different keys of list[] and puts the K best into won[] in order (won[] beyond m: 0).
+__device__ __forceinline__ void beam_rank(const unsigned long long* list, int m, unsigned long long* won, int K, int lane) {
+  if (lane < K) won[lane] = 0;
+  const unsigned long long a = lane < m ? list[lane] : 0;
+  int ra = 0;
   if (m <= 64) {
+#pragma unroll 4
     for (int j = 0; j < m; ++j) ra += list[j] > a;
   } else {
+    const unsigned long long b = lane + 64 < m ? list[lane + 64] : 0;
+    int rb = 0;
+#pragma unroll 4
     for (int j = 0; j < m; ++j) {
       const unsigned long long o = list[j];
       ra += o > a;
       rb += o > b;
     }
+    if (lane + 64 < m && rb < K) won[rb] = b;
   }
   wave_sync();
-  if (lane < m && ra < keep) won[ra] = a;
-  if (lane + 64 < m && rb < keep) won[rb] = b;
+  if (lane < m && ra < K) won[ra] = a;
   wave_sync();
 }
 
-// The K best of a wave's N orders per lane (0: nothing) into won[0 .. K) (keys; 0 where there are fewer), by way of list[],
-// room for 128.  index(i) is the index of a lane's i-th element.  above: only orders greater than it count.
-// What reaches the bound is nearly always few; where it is not (ties all over) the keys are taken out one by one.
+// The K best of a wave's N numbers per lane, those above `above` only (-inf: all), and of the `m` keys that list[] (room for
+// 128) already holds, into won[0 .. K) by rank (keys; 0 where there are fewer).  index(i): of a lane's i-th number.
+// best: the lane's largest number.  What reaches the bound is nearly always few; where it is not (ties all over) the keys are
+// taken out one by one.
 template <int N, class F>
-__device__ __forceinline__ void beam_best(const unsigned (&order)[N], F index, unsigned above, int K, unsigned long long* list,
+__device__ __forceinline__ void beam_best(const float (&c)[N], F index, float best, float above, int K, unsigned long long* list, int m,
                                           unsigned long long* won, int lane) {
-  unsigned best = 0;
+  const int some = __popcll(__ballot(best > above));
+  float bound = some > K ? beam_bound(best, above, K) : beam_unorder(beam_order(above) + 1);
+  const int m0 = m;
+  // A few lanes may hold most of what reaches the bound (rows of very different scores): then halve by numbers, not by lanes.
+  if (some > K) {
+    int all = 0;
 #pragma unroll
-  for (int i = 0; i < N; ++i) best = max(best, order[i]);
-  if (best <= above) best = 0;
-  const unsigned bound = max(beam_bound(best, K), above + 1);
-  int m = 0;
+    for (int i = 0; i < N; ++i) all += __popcll(__ballot(c[i] >= bound));
+    unsigned lo = beam_order(bound), hi = beam_order(max64(best)) + 1;
+    while (all > 64 && hi - lo > 1) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      const float f = beam_unorder(mid);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) n += __popcll(__ballot(c[i] >= f));
+      if (n >= K) { lo = mid; all = n; }
+      else hi = mid;
+    }
+    bound = beam_unorder(lo);
+  }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const bool in = order[i] >= bound;
+    const bool in = c[i] >= bound;
     const unsigned long long b = __ballot(in);
     if (b) {
       const int at = m + lanes_before(b);
-      if (in && at < 128) list[at] = beam_key(order[i], index(i));
+      if (in && at < 128) list[at] = beam_key(c[i], index(i));
       m += __popcll(b);
     }
   }
@@ -191,10 +232,11 @@ __device__ __forceinline__ void beam_best(const unsigned (&order)[N], F index, u
   unsigned long long last = ~0ull;
   for (int j = 0; j < K; ++j) {
     unsigned long long top = 0;
+    if (lane < m0 && list[lane] < last) top = list[lane];           // (m0 <= 64)
     if (last) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const unsigned long long k = order[i] >= bound ? beam_key(order[i], index(i)) : 0;
+        const unsigned long long k = c[i] >= bound ? beam_key(c[i], index(i)) : 0;
         if (k < last && k > top) top = k;
       }
     }
@@ -205,15 +247,15 @@ __device__ __forceinline__ void beam_best(const unsigned (&order)[N], F index, u
 }
 
 // ---- the step's outputs -----------------------------------------------------------------------------------------------
-// One wave; won[] holds the group's K keys by rank (order of c, index k * V + v), fin the finished beams as bits.
+// One wave; won[] holds the group's K keys by rank, fin the finished beams as bits.
 // keep: the best child of a beam takes the beam's place (won[] is by rank, so it is the lowest lane that names the parent),
 // the others take the free places in ascending order, then come the entries without a candidate.  place[]: room for K.
 __device__ __forceinline__ void beam_write(const BeamSelect& a, long g, const unsigned long long* won, unsigned fin, int* place,
                                            int lane) {
   const int K = a.K;
   const unsigned long long key = lane < K ? won[lane] : 0;
-  const unsigned flat = beam_key_index(key);
-  const int parent = key ? (int)(flat / (unsigned)a.V) : -1, v = key ? (int)(flat % (unsigned)a.V) : a.pad;
+  const unsigned index = beam_key_index(key);
+  const int parent = key ? (int)(index >> 20) : -1, v = key ? (int)(index & 0xFFFFFu) : a.pad;
   int to = lane;
   if (a.keep) {
     unsigned long long first = 0;

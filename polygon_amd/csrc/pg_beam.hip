@@ -3,86 +3,103 @@
 #include "pg_beam.h"
 #include "pg_host.h"
 
-// ---- short vocabularies (V <= 128): one wave per group ---------------------------------------------------------------
-// 16 lanes hold a row (E = 4 or 8 neighbouring symbols per lane, one wide load), 4 rows at a time, P times: the whole group
-// stays in registers (at most 64 of them), so the logits are read once, and all reductions are inside 16 lanes (DPP).
-constexpr int SW = 4;      // waves (groups) per workgroup
-template <typename T, int E, int P>
+// ---- short vocabularies (V <= 128) ------------------------------------------------------------------------------------
+// 16 lanes hold a row (E = 4 or 8 neighbouring symbols per lane, one wide load), a wave 4 rows at a time, P <= 2 times: a wave
+// takes up to 8 of a group's rows and a group G = 1, 2 or 4 waves.  The logits are read once and stay in registers (at most 16
+// of them), all of softmax's reductions are inside 16 lanes (DPP).  With G > 1 the first wave selects from the G waves' best.
+// Bound by instructions: about half of them the selection, a quarter the 64-bit exponentials.
+constexpr int SW = 4;      // waves per workgroup
+template <typename T, int E, int P, int G>
 __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a) {
   __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
-  __shared__ double sum_s[SW][PG_MAX_BEAMS];
+  __shared__ double sum_s[SW][4 * P];
   __shared__ int place_s[SW][PG_MAX_BEAMS];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long g = (long)blockIdx.x * SW + __builtin_amdgcn_readfirstlane(wave);
-  if (g >= a.n) return;                       // no barrier below: waves are on their own
-  const int K = a.K, V = a.V, sub = lane & 15, v0 = sub * E;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const long g = ((long)blockIdx.x * SW + wave) / G;
+  if (G == 1 && g >= a.n) return;             // (G > 1: such a wave has no open beam, and takes part in the barrier)
+  const int K = a.K, V = a.V, k0 = wave % G * (4 * P), row = lane >> 4;
   // beam `lane`
   float s_mine = -INFINITY;
   bool fin_mine = false;
-  if (lane < K) {
+  if (lane < K && (G == 1 || g < a.n)) {
     s_mine = a.scores[g * K + lane];
     fin_mine = a.finished && a.finished[g * K + lane];
   }
   const unsigned fin = (unsigned)__ballot(fin_mine), alive = (unsigned)__ballot(isfinite(s_mine)), open = alive & ~fin;
-  const T* x0 = (const T*)a.logits + g * a.ld_group;
+  // the lane's symbols v0 .. v0+E-1 of its rows; the row's last lane reads the last E, and leaves out those it shares
+  const int sub = (lane & 15) * E, v0 = min(sub, max(V - E, 0));
   float x[P][E], m[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    const int k = p * 4 + (lane >> 4);
+    const int k = k0 + p * 4 + row;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[p][e] = -INFINITY;
-    if (!(open >> k & 1) || v0 >= V) continue;
-    const T* r = x0 + k * a.ld_row + v0;
+    if (!(open >> k & 1) || sub >= V) continue;
+    const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row + v0;
     const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row + v0 : nullptr;
-    if (v0 + E <= V) {
+    if (V >= E) {
       T t[E];
       __builtin_memcpy(t, r, sizeof(t));
-      uint8_t ok[E];
-      if (mk) __builtin_memcpy(ok, mk, E);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[p][e] = !mk || ok[e] ? to_f32<T>(t[e]) : -INFINITY;
+      for (int e = 0; e < E; ++e) x[p][e] = v0 + e >= sub ? to_f32<T>(t[e]) : -INFINITY;
+      if (mk) {
+        uint8_t ok[E];
+        __builtin_memcpy(ok, mk, E);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (!ok[e]) x[p][e] = -INFINITY;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if (v0 + e < V && (!mk || mk[e])) x[p][e] = to_f32<T>(r[e]);
+        if (e < V && (!mk || mk[e])) x[p][e] = to_f32<T>(r[e]);
     }
   }
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    float mx = -INFINITY;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      bad |= !(x[p][e] < INFINITY);            // NaN or +inf: the row's maximum becomes +inf, and the beam has no continuation
-      mx = fmaxf(mx, x[p][e]);
-    }
-    m[p] = max16(bad ? INFINITY : mx);
+    const float mx = max_nan(x[p]);
+    m[p] = max16(mx != mx ? INFINITY : mx);    // a NaN or +inf makes the row's maximum +inf, and the beam has no continuation
     double sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += beam_exp(((double)x[p][e] - (double)m[p]) * a.inv_temp);
+    for (int e = 0; e < E; ++e) sum += beam_exp2(((double)x[p][e] - (double)m[p]) * a.scale);
     sum = sum16(sum);
-    if (sub == 0) sum_s[wave][p * 4 + (lane >> 4)] = sum;
+    if ((lane & 15) == 0) sum_s[wave][p * 4 + row] = sum;
   }
   wave_sync();
   // one logarithm for all rows
-  if (lane < P * 4) sum_s[wave][lane] = log(sum_s[wave][lane]);
+  if (lane < 4 * P) sum_s[wave][lane] = beam_log(sum_s[wave][lane]);
   wave_sync();
-  unsigned order[P * E];
+  float c[P * E], best = -INFINITY;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    const int k = p * 4 + (lane >> 4);
+    const int k = k0 + p * 4 + row;
     const float s = __shfl(s_mine, k);
-    const double lse = sum_s[wave][k];
+    const double lse = sum_s[wave][p * 4 + row];
     const bool has = (open >> k & 1) && isfinite(m[p]), done = alive & fin & (1u << k);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float c = has ? beam_score(x[p][e], m[p], a.inv_temp, lse, s) : -INFINITY;
-      if (done && v0 + e == a.pad) c = s + 0.0f;
-      order[p * E + e] = c > -INFINITY ? beam_order(c) : 0;
+      float f = has ? beam_score(x[p][e], m[p], a.inv_temp, lse, s) : -INFINITY;
+      if (done && v0 + e == a.pad && v0 + e >= sub) f = s;
+      c[p * E + e] = f;
+      best = fmaxf(best, f);
     }
   }
-  beam_best<P * E>(order, [&](int i) { return (unsigned)((i / E * 4 + (lane >> 4)) * V + v0 + i % E); }, 0, K, list_s[wave],
-                   won_s[wave], lane);
+  beam_best<P * E>(c, [&](int i) { return (unsigned)(k0 + i / E * 4 + row) << 20 | (unsigned)(v0 + i % E); }, best, -INFINITY, K,
+                   list_s[wave], 0, won_s[wave], lane);
+  if (G > 1) {
+    __syncthreads();
+    if (wave % G != 0 || g >= a.n) return;
+    float t[G], top = -INFINITY;
+    unsigned at[G];
+#pragma unroll
+    for (int w = 0; w < G; ++w) {
+      const unsigned long long key = lane < K ? won_s[wave + w][lane] : 0;
+      t[w] = key ? beam_key_number(key) : -INFINITY;
+      at[w] = beam_key_index(key);
+      top = fmaxf(top, t[w]);
+    }
+    beam_best<G>(t, [&](int i) { return at[i]; }, top, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
+  }
   beam_write(a, g, won_s[wave], fin, place_s[wave], lane);
 }
 
@@ -115,63 +132,57 @@ __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamL
   const int k = (int)(row - g * K);
   const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row;
   const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row : nullptr;
+  constexpr int W = 16 / sizeof(T);
   float mx = -INFINITY;
   double sum = 0.0;
   bool bad = false;
-  unsigned above = 0;            // order of the K-th best so far (0: fewer than K)
+  float above = -INFINITY;       // the K-th best so far (-inf: fewer than K)
   unsigned long long mine = 0;   // lane j: the j-th best key so far
   for (int t = 0; t < l.tiles; ++t) {
     const long b = ((long)chunk * l.tiles + t) * TILE;
     if (b >= V) break;
+    // 16-byte loads: W = 4 (fp32) or 8 (bf16) neighbouring symbols per lane and load, a wave's loads dense, all in flight together
     float x[LE];
-    // 16-byte loads: 4 (fp32) or 8 (bf16) neighbouring symbols per lane and load, a wave's loads dense
-    constexpr int W = 16 / sizeof(T);
+    if (b + TILE <= V) {
+      T e[LE];
 #pragma unroll
-    for (int q = 0; q < LE / W; ++q) {
-      const long v = b + (q * 64 + lane) * W;
-      if (v + W <= V) {
-        T e[W];
-        __builtin_memcpy(e, r + v, sizeof(e));
-        uint8_t ok[W];
-        if (mk) __builtin_memcpy(ok, mk + v, W);
+      for (int q = 0; q < LE / W; ++q) __builtin_memcpy(e + q * W, r + b + (q * 64 + lane) * W, 16);
+      if (mk) {
+        uint8_t ok[LE];
 #pragma unroll
-        for (int i = 0; i < W; ++i) x[q * W + i] = !mk || ok[i] ? to_f32<T>(e[i]) : -INFINITY;
+        for (int q = 0; q < LE / W; ++q) __builtin_memcpy(ok + q * W, mk + b + (q * 64 + lane) * W, W);
+#pragma unroll
+        for (int i = 0; i < LE; ++i) x[i] = ok[i] ? to_f32<T>(e[i]) : -INFINITY;
       } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) x[q * W + i] = v + i < V && (!mk || mk[v + i]) ? to_f32<T>(r[v + i]) : -INFINITY;
+        for (int i = 0; i < LE; ++i) x[i] = to_f32<T>(e[i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LE; ++i) {
+        const long v = b + (i / W * 64 + lane) * W + i % W;
+        x[i] = v < V && (!mk || mk[v]) ? to_f32<T>(r[v]) : -INFINITY;
       }
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < LE; ++i) {
-      bad |= !(x[i] < INFINITY);
-      top = fmaxf(top, x[i]);
-    }
+    const float top = max_nan(x);
+    bad |= top != top || top == INFINITY;
     const float all = max64(top);
     if (!(all > -INFINITY) || all == INFINITY) continue;
     if (all > mx) {
-      sum *= beam_exp(((double)mx - (double)all) * a.inv_temp);
+      sum *= beam_exp2(((double)mx - (double)all) * a.scale);
       mx = all;
     }
 #pragma unroll
-    for (int i = 0; i < LE; ++i) sum += beam_exp(((double)x[i] - (double)mx) * a.inv_temp);
-    if (!__ballot(top > -INFINITY && beam_order(top) > above)) continue;
-    unsigned order[LE];
-#pragma unroll
-    for (int i = 0; i < LE; ++i) order[i] = x[i] > -INFINITY ? beam_order(x[i]) : 0;
-    beam_best<LE>(order, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, above, K, list_s[wave], won_s[wave],
-                  lane);
-    if (t == 0) mine = lane < K ? won_s[wave][lane] : 0;
-    else {   // the K best of two lists of K
-      if (lane < K) list_s[wave][lane] = won_s[wave][lane];
-      const unsigned long long old = __ballot(mine != 0), fresh = __ballot(lane < K && won_s[wave][lane] != 0);
-      const int nf = __popcll(fresh);
-      if (mine) list_s[wave][nf + lanes_before(old)] = mine;
-      wave_sync();
-      beam_rank(list_s[wave], nf + __popcll(old), won_s[wave], K, lane);
-      mine = lane < K ? won_s[wave][lane] : 0;
-    }
-    above = __builtin_amdgcn_readlane((int)(mine >> 32), K - 1);
+    for (int i = 0; i < LE; ++i) sum += beam_exp2(((double)x[i] - (double)mx) * a.scale);
+    if (!__ballot(top > above)) continue;
+    // the K best so far first, then what this tile has above the last of them
+    const unsigned long long old = __ballot(mine != 0);
+    if (mine) list_s[wave][lane] = mine;
+    beam_best<LE>(x, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, top, above, K, list_s[wave], __popcll(old),
+                  won_s[wave], lane);
+    mine = lane < K ? won_s[wave][lane] : 0;
+    const unsigned kth = __builtin_amdgcn_readlane((int)(mine >> 32), K - 1);
+    above = kth ? beam_unorder(kth) : -INFINITY;
   }
   const bool any_bad = __ballot(bad) != 0;
   sum = sum64(sum);
@@ -206,10 +217,10 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
       for (int c = lane; c < l.chunks; c += 64) mx = fmaxf(mx, part[c].max);
       mx = max64(mx);
       if (isfinite(mx))
-        for (int c = lane; c < l.chunks; c += 64) sum += part[c].sum * beam_exp(((double)part[c].max - (double)mx) * a.inv_temp);
+        for (int c = lane; c < l.chunks; c += 64) sum += part[c].sum * beam_exp2(((double)part[c].max - (double)mx) * a.scale);
       sum = sum64(sum);
     }
-    if (lane == 0) { max_s[k] = mx; lse_s[k] = log(sum); }
+    if (lane == 0) { max_s[k] = mx; lse_s[k] = beam_log(sum); }
   }
   if (tid == 0) have = 0;
   __syncthreads();
@@ -222,10 +233,10 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     const unsigned long long key = keys[e];
     if (!key) return 0;
     const float c = beam_score(beam_key_number(key), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
-    return c > -INFINITY ? beam_key(beam_order(c), (unsigned)(k * V) + beam_key_index(key)) : 0;
+    return c > -INFINITY ? beam_key(c, (unsigned)k << 20 | beam_key_index(key)) : 0;
   };
   auto ended = [&](int k) -> unsigned long long {      // a finished beam's own candidate
-    return alive & fin & (1u << k) ? beam_key(beam_order(score_s[k] + 0.0f), (unsigned)(k * V + a.pad)) : 0;
+    return alive & fin & (1u << k) ? beam_key(score_s[k], (unsigned)k << 20 | (unsigned)a.pad) : 0;
   };
   // a bound that at least K of the threads' bests reach (found in every wave alike)
   unsigned best = tid < K ? (unsigned)(ended(tid) >> 32) : 0;
@@ -312,7 +323,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     {
       const int kc = base + tid;       // (beam, chunk); one that starts behind the last winner cannot hold a lower index
       if (kc < K * l.chunks && (unsigned)(entry(kc * K + K - 1) >> 32) == edge &&
-          (unsigned)(kc / l.chunks * V) + (unsigned)(kc % l.chunks) * l.tiles * TILE < beam_key_index(won[K - 1]))
+          ((unsigned)(kc / l.chunks) << 20 | (unsigned)(kc % l.chunks) * l.tiles * TILE) < beam_key_index(won[K - 1]))
         again[atomicAdd(&have, 1)] = kc;
     }
     __syncthreads();
@@ -329,8 +340,8 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
         for (long v = (long)c * l.tiles * TILE + tid; v < v1; v += 64 * JW) {
           if (mk && !mk[v]) continue;
           const float sc = beam_score(to_f32<T>(r[v]), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
-          if (!(sc > -INFINITY) || beam_order(sc) != edge) continue;
-          const unsigned long long key = beam_key(edge, (unsigned)(k * V + v));
+          const unsigned long long key = beam_key(sc, (unsigned)k << 20 | (unsigned)v);
+          if ((unsigned)(key >> 32) != edge) continue;
           if (key < last && key > top) top = key;
         }
         top = max64(top);
@@ -379,10 +390,9 @@ extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V)
 
 template <typename T> static int beam_select_t(const BeamSelect& a, void* ws, size_t ws_bytes, hipStream_t st) {
   if (a.V <= SHORT_V) {
-    const dim3 grid(cdiv(a.n, SW)), block(64 * SW);
-#define PG_SHORT(E, P) hipLaunchKernelGGL((beam_select_short_kernel<T, E, P>), grid, block, 0, st, a)
+#define PG_SHORT(E, P, G) hipLaunchKernelGGL((beam_select_short_kernel<T, E, P, G>), dim3(cdiv((long)a.n * G, SW)), dim3(64 * SW), 0, st, a)
 #define PG_SHORT_E(E) \
-  do { if (a.K <= 4) PG_SHORT(E, 1); else if (a.K <= 8) PG_SHORT(E, 2); else if (a.K <= 16) PG_SHORT(E, 4); else PG_SHORT(E, 8); } while (0)
+  do { if (a.K <= 4) PG_SHORT(E, 1, 1); else if (a.K <= 8) PG_SHORT(E, 2, 1); else if (a.K <= 16) PG_SHORT(E, 2, 2); else PG_SHORT(E, 2, 4); } while (0)
     if (a.V <= 64) PG_SHORT_E(4);
     else PG_SHORT_E(8);
 #undef PG_SHORT_E
@@ -411,12 +421,12 @@ extern "C" int pg_beam_select(int dtype, const void* logits, long ld_group, long
   PG_REQUIRE(dtype == PG_F32 || dtype == PG_BF16, "pg_beam_select: dtype %d is neither PG_F32 nor PG_BF16", dtype);
   PG_REQUIRE(n >= 0 && K >= 1 && K <= PG_MAX_BEAMS && V >= 1 && V <= PG_MAX_BEAM_V,
              "pg_beam_select: n=%d, K=%d outside [1,%d] or V=%d outside [1,%d]", n, K, PG_MAX_BEAMS, V, PG_MAX_BEAM_V);
-  PG_REQUIRE(temp > 0.0 && isfinite(temp) && isfinite(1.0 / temp), "pg_beam_select: temperature must be positive and finite");
+  PG_REQUIRE(temp > 0.0 && isfinite(temp) && isfinite(2.0 / temp), "pg_beam_select: temperature must be positive and finite");
   PG_REQUIRE(pad >= 0 && pad < V && eos < V, "pg_beam_select: pad=%d outside [0,%d) or eos=%d not below it", pad, V, eos);
-  PG_REQUIRE((long)n * K <= 1L << 26, "pg_beam_select: n * K = %ld above 2^26", (long)n * K);
+  PG_REQUIRE((long)n * K < 1L << 24, "pg_beam_select: n * K = %ld is not below 2^24", (long)n * K);
   if (n == 0) return PG_OK;
   PG_REQUIRE(logits && scores && scores_out && parents && tokens && finished_out, "pg_beam_select: NULL buffer");
-  const BeamSelect a = {logits, ld_group, ld_row, n, K, V, mask, mask_group, mask_row, 1.0 / temp, scores, finished, eos, pad, keep_slots,
+  const BeamSelect a = {logits, ld_group, ld_row, n, K, V, mask, mask_group, mask_row, 1.0 / temp, BEAM_LOG2E / temp, scores, finished, eos, pad, keep_slots,
                         scores_out, parents, tokens, finished_out};
   return dtype == PG_BF16 ? beam_select_t<bf16_t>(a, ws, ws_bytes, (hipStream_t)stream)
                           : beam_select_t<float>(a, ws, ws_bytes, (hipStream_t)stream);
