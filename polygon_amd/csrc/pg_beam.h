@@ -38,6 +38,7 @@ __device__ __forceinline__ float beam_key_number(unsigned long long k) { return 
 // to the least largest relative error of 2^f on that interval, 8.1e-13 (Lawson's iteration), n added to the exponent.  13
 // instructions, all at the full 64-bit rate, which is also that of fp32 here.  Which candidate wins hangs on the normaliser:
 // 32 bits (6e-8) would let near ties flip, 8e-13 is a millionth of what a score's rounding to fp32 can tell.  2^0 is exactly 1.
+typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 constexpr double BEAM_LOG2E = 1.4426950408889634074;
 __device__ __forceinline__ double beam_exp2(double t) {
   t = fmax(t, -1000.0);                      // -inf and all that would underflow: 1e-301
@@ -51,9 +52,9 @@ __device__ __forceinline__ double beam_exp2(double t) {
   p = fma(p, f, 2.4022650698110698366e-1);
   p = fma(p, f, 6.9314718054821182051e-1);
   p = fma(p, f, 1.0);
-  const long long b = __double_as_longlong(p);
-  const unsigned hi = (unsigned)(b >> 32) + ((unsigned)__double_as_longlong(big) << 20);
-  return __longlong_as_double(((long long)hi << 32) | (unsigned)b);
+  u32x2 b = __builtin_bit_cast(u32x2, p);
+  b.y += __builtin_bit_cast(u32x2, big).x << 20;
+  return __builtin_bit_cast(double, b);
 }
 // ln of a softmax's sum, 1 <= z <= 2^20: the hardware's log2 (a few 1e-7 off) corrected once by what z falls short of its power,
 // ln z = y ln 2 + ln(z 2^-y), the last factor within 1e-6 of 1.  As exact as beam_exp2; ln 1 is exactly 0.
@@ -197,13 +198,26 @@ __device__ __forceinline__ void beam_best(const float (&c)[N], F index, float be
   const int some = __popcll(__ballot(best > above));
   float bound = some > K ? beam_bound(best, above, K) : beam_unorder(beam_order(above) + 1);
   const int m0 = m;
-  // A few lanes may hold most of what reaches the bound (rows of very different scores): then halve by numbers, not by lanes.
-  if (some > K) {
-    int all = 0;
+  auto put = [&]() {
+    m = m0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) all += __popcll(__ballot(c[i] >= bound));
+    for (int i = 0; i < N; ++i) {
+      const bool in = c[i] >= bound;
+      const unsigned long long b = __ballot(in);
+      if (b) {
+        const int at = m + lanes_before(b);
+        if (in && at < 128) list[at] = beam_key(c[i], index(i));
+        m += __popcll(b);
+      }
+    }
+    wave_sync();
+  };
+  put();
+  if (m > 128) {
+    // a few lanes hold most of it (rows of very different scores): halve by numbers instead of lanes
     unsigned lo = beam_order(bound), hi = beam_order(max64(best)) + 1;
-    while (all > 64 && hi - lo > 1) {
+    int all = m - m0;
+    while (all + m0 > 128 && hi - lo > 1) {
       const unsigned mid = lo + (hi - lo) / 2;
       const float f = beam_unorder(mid);
       int n = 0;
@@ -213,35 +227,35 @@ __device__ __forceinline__ void beam_best(const float (&c)[N], F index, float be
       else hi = mid;
     }
     bound = beam_unorder(lo);
+    if (all + m0 <= 128) put();
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const bool in = c[i] >= bound;
-    const unsigned long long b = __ballot(in);
-    if (b) {
-      const int at = m + lanes_before(b);
-      if (in && at < 128) list[at] = beam_key(c[i], index(i));
-      m += __popcll(b);
-    }
-  }
-  wave_sync();
   if (m <= 128) {
     beam_rank(list, m, won, K, lane);
     return;
   }
-  unsigned long long last = ~0ull;
+  // (rare: written so that it needs no registers of its own - `zero` keeps the indices from being worked out ahead of the loop)
+  float last = INFINITY;
+  unsigned last_i = 0;
+  const unsigned long long held = lane < m0 ? list[lane] : 0;           // (m0 <= 64)
   for (int j = 0; j < K; ++j) {
-    unsigned long long top = 0;
-    if (lane < m0 && list[lane] < last) top = list[lane];           // (m0 <= 64)
-    if (last) {
+    unsigned zero = 0;
+    asm volatile("" : "+v"(zero));
+    auto next = [&](float f, unsigned i) { return f < last || (f == last && i > last_i); };
+    float top = -INFINITY;
+    if (held && next(beam_key_number(held), beam_key_index(held))) top = beam_key_number(held);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const unsigned long long k = c[i] >= bound ? beam_key(c[i], index(i)) : 0;
-        if (k < last && k > top) top = k;
-      }
-    }
-    last = max64(top);
-    if (lane == 0) won[j] = last;
+    for (int i = 0; i < N; ++i)
+      if (c[i] >= bound && next(c[i], index(i) + zero)) top = fmaxf(top, c[i]);
+    top = max64(top);
+    unsigned top_i = 0xFFFFFFFFu;
+    if (held && beam_key_number(held) == top && next(top, beam_key_index(held))) top_i = beam_key_index(held);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c[i] == top && next(top, index(i) + zero)) top_i = min(top_i, index(i) + zero);
+    for (int o = 32; o; o >>= 1) top_i = min(top_i, (unsigned)__shfl_xor(top_i, o));
+    if (lane == 0) won[j] = top > -INFINITY ? beam_key(top, top_i) : 0;
+    last = top;
+    last_i = top_i;
   }
   wave_sync();
 }

@@ -104,23 +104,23 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
 }
 
 // ---- long vocabularies ------------------------------------------------------------------------------------------------
-// The vocabulary is split into chunks; a wave walks through its chunk in tiles of 64 x 16 symbols held in registers, with a
+// The vocabulary is split into chunks; a wave walks through its chunk in tiles of 64 x 8 or 16 symbols held in registers, with a
 // running maximum and 64-bit sum of the softmax and the K best logits so far (a tile's symbols at or below the K-th best are
 // out at one comparison per lane).  A chunk leaves (max, sum, K keys of logit and symbol).  A workgroup per group then joins
 // the chunks' sums, turns their keys into scores and selects.
-constexpr int LE = 16, TILE = 64 * LE;
 struct BeamChunk {
   double sum;
   float max;       // +inf: a NaN or +inf was seen
   int pad;
 };
 struct BeamLong {
-  int chunks, tiles;             // per row; tiles per chunk
+  int tile, tiles, chunks;       // symbols of a tile; tiles of a chunk; chunks of a row
   BeamChunk* part;               // [n * K, chunks]
   unsigned long long* keys;      // [n * K, chunks, K]
 };
-template <typename T>
+template <typename T, int LE>
 __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamLong l) {
+  constexpr int TILE = 64 * LE;
   __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long u = (long)blockIdx.x * SW + __builtin_amdgcn_readfirstlane(wave);
@@ -137,7 +137,16 @@ __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamL
   double sum = 0.0;
   bool bad = false;
   float above = -INFINITY;       // the K-th best so far (-inf: fewer than K)
-  unsigned long long mine = 0;   // lane j: the j-th best key so far
+  unsigned long long *list = list_s[wave], *won = won_s[wave];
+  int m = 0;                     // keys in list[], at most 48 between tiles: the K best when it was last ranked, and later ones
+  auto settle = [&]() {          // won[] becomes the list
+    const unsigned long long key = lane < K ? won[lane] : 0;
+    if (key) list[lane] = key;
+    m = __popcll(__ballot(key != 0));
+    const unsigned kth = __builtin_amdgcn_readlane((int)(key >> 32), K - 1);
+    above = kth ? beam_unorder(kth) : -INFINITY;
+    wave_sync();
+  };
   for (int t = 0; t < l.tiles; ++t) {
     const long b = ((long)chunk * l.tiles + t) * TILE;
     if (b >= V) break;
@@ -173,24 +182,42 @@ __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamL
       mx = all;
     }
 #pragma unroll
-    for (int i = 0; i < LE; ++i) sum += beam_exp2(((double)x[i] - (double)mx) * a.scale);
+    for (int i = 0; i < LE; ++i) {
+      sum += beam_exp2(((double)x[i] - (double)mx) * a.scale);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // four at a time: enough to hide their latency, and few registers
+    }
     if (!__ballot(top > above)) continue;
-    // the K best so far first, then what this tile has above the last of them
-    const unsigned long long old = __ballot(mine != 0);
-    if (mine) list_s[wave][lane] = mine;
-    beam_best<LE>(x, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, top, above, K, list_s[wave], __popcll(old),
-                  won_s[wave], lane);
-    mine = lane < K ? won_s[wave][lane] : 0;
-    const unsigned kth = __builtin_amdgcn_readlane((int)(mine >> 32), K - 1);
-    above = kth ? beam_unorder(kth) : -INFINITY;
+    // what the tile has above the K-th best is put behind the K best, and the list is ranked when it has grown: a stale bound
+    // lets a few more in, which is cheaper than a ranking per tile
+    const int m0 = m;
+    if (__popcll(__ballot(top > above)) <= 32) {
+#pragma unroll
+      for (int i = 0; i < LE; ++i) {
+        const bool in = x[i] > above;
+        const unsigned long long some = __ballot(in);
+        if (some) {
+          const int at = m + lanes_before(some);
+          if (in && at < 128) list[at] = beam_key(x[i], (unsigned)(b + (i / W * 64 + lane) * W + i % W));
+          m += __popcll(some);
+        }
+      }
+      if (m <= 48) continue;
+    }
+    if (m > m0 && m <= 128) beam_rank(list, m, won, K, lane);
+    else beam_best<LE>(x, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, top, above, K, list, m0, won, lane);
+    settle();
   }
+  if (m > K) { beam_rank(list, m, won, K, lane); settle(); }
   const bool any_bad = __ballot(bad) != 0;
   sum = sum64(sum);
   if (lane == 0) l.part[row * l.chunks + chunk] = {sum, any_bad ? INFINITY : mx, 0};
-  if (lane < K) l.keys[(row * l.chunks + chunk) * K + lane] = mine;
+  if (lane < K) l.keys[(row * l.chunks + chunk) * K + lane] = lane < m ? list[lane] : 0;
 }
 
-constexpr int JW = 4, JLIST = 1024;
+// One workgroup per group.  The first JKEEP entries of every thread are loaded before anything else and stay in registers (that
+// is all of them unless K * K * chunks > 2048), their latency behind the rows' sums, which 16 lanes each work out.
+// Bound by latency: a chain of loads, two exchanges through LDS, and the ranking of some 2 K keys.
+constexpr int JW = 4, JLIST = 1024, JKEEP = 8;
 template <typename T>
 __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLong l) {
   __shared__ unsigned long long list[JLIST], won[PG_MAX_BEAMS], red[JW];
@@ -200,6 +227,8 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   __shared__ unsigned best_s[64 * JW];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, K = a.K, V = a.V;
   const long g = blockIdx.x;
+  const int per_row = l.chunks * K, total = K * per_row;
+  const unsigned long long* keys = l.keys + g * (long)total;
   float s_mine = -INFINITY;
   bool fin_mine = false;
   if (lane < K) {
@@ -207,40 +236,54 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     fin_mine = a.finished && a.finished[g * K + lane];
   }
   const unsigned fin = (unsigned)__ballot(fin_mine), alive = (unsigned)__ballot(isfinite(s_mine)), open = alive & ~fin;
+  // (a row that is not open was not written: its entries are not looked at)
+  unsigned long long kept[JKEEP];
+#pragma unroll
+  for (int i = 0; i < JKEEP; ++i) {
+    const int e = tid + i * 64 * JW;
+    kept[i] = e < total && (open >> (e / per_row) & 1) ? keys[e] : 0;
+  }
   if (wave == 0 && lane < K) score_s[lane] = s_mine;
-  // every row's maximum and normaliser from its chunks
-  for (int k = wave; k < K; k += JW) {
+  // every row's maximum and normaliser from its chunks, 16 lanes a row
+  for (int k0 = wave * 4; k0 < K; k0 += 4 * JW) {
+    const int k = k0 + (lane >> 4), c0 = lane & 15;
+    const bool here = open >> k & 1;          // (false for k >= K)
+    const BeamChunk* part = l.part + (g * K + k) * l.chunks;
     float mx = -INFINITY;
     double sum = 0.0;
-    if (open >> k & 1) {
-      const BeamChunk* part = l.part + (g * K + k) * l.chunks;
-      for (int c = lane; c < l.chunks; c += 64) mx = fmaxf(mx, part[c].max);
-      mx = max64(mx);
-      if (isfinite(mx))
-        for (int c = lane; c < l.chunks; c += 64) sum += part[c].sum * beam_exp2(((double)part[c].max - (double)mx) * a.scale);
-      sum = sum64(sum);
-    }
-    if (lane == 0) { max_s[k] = mx; lse_s[k] = beam_log(sum); }
+    if (here)
+      for (int c = c0; c < l.chunks; c += 16) mx = fmaxf(mx, part[c].max);
+    mx = max16(mx);
+    if (here && isfinite(mx))
+      for (int c = c0; c < l.chunks; c += 16) sum += part[c].sum * beam_exp2(((double)part[c].max - (double)mx) * a.scale);
+    sum = sum16(sum);
+    if (c0 == 0 && k < K) { max_s[k] = mx; lse_s[k] = beam_log(sum); }
   }
   if (tid == 0) have = 0;
   __syncthreads();
-  // an entry's score, or 0: entry e of the group's K * chunks * K
-  const int per_row = l.chunks * K, total = K * per_row;
-  const unsigned long long* keys = l.keys + g * (long)total;
-  auto entry = [&](int e) -> unsigned long long {
+  // entry e of the group's K * chunks * K, as a key of its score (0: none)
+  auto scored = [&](int e, unsigned long long key) -> unsigned long long {
     const int k = e / per_row;
-    if (!(open >> k & 1) || !isfinite(max_s[k])) return 0;
-    const unsigned long long key = keys[e];
-    if (!key) return 0;
+    if (!key || !isfinite(max_s[k])) return 0;
     const float c = beam_score(beam_key_number(key), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
     return c > -INFINITY ? beam_key(c, (unsigned)k << 20 | beam_key_index(key)) : 0;
   };
+  auto entry = [&](int e) -> unsigned long long { return open >> (e / per_row) & 1 ? scored(e, keys[e]) : 0; };
   auto ended = [&](int k) -> unsigned long long {      // a finished beam's own candidate
     return alive & fin & (1u << k) ? beam_key(score_s[k], (unsigned)k << 20 | (unsigned)a.pad) : 0;
   };
+#pragma unroll
+  for (int i = 0; i < JKEEP; ++i)
+    if (tid + i * 64 * JW < total) kept[i] = scored(tid + i * 64 * JW, kept[i]);
+  auto each = [&](auto f) {
+    if (tid < K) f(ended(tid));
+#pragma unroll
+    for (int i = 0; i < JKEEP; ++i) f(kept[i]);
+    for (int e = tid + JKEEP * 64 * JW; e < total; e += 64 * JW) f(entry(e));
+  };
   // a bound that at least K of the threads' bests reach (found in every wave alike)
-  unsigned best = tid < K ? (unsigned)(ended(tid) >> 32) : 0;
-  for (int e = tid; e < total; e += 64 * JW) best = max(best, (unsigned)(entry(e) >> 32));
+  unsigned best = 0;
+  each([&](unsigned long long key) { best = max(best, (unsigned)(key >> 32)); });
   best_s[tid] = best;
   __syncthreads();
   unsigned b4[JW], bound = 1;
@@ -279,8 +322,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     const int at = atomicAdd(&have, 1);       // the list's order does not matter: its keys are ranked
     if (at < JLIST) list[at] = key;
   };
-  if (tid < K) put(ended(tid));
-  for (int e = tid; e < total; e += 64 * JW) put(entry(e));
+  each(put);
   if (tid < K) won[tid] = 0;
   __syncthreads();
   const int m = have;
@@ -295,9 +337,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     unsigned long long last = ~0ull;
     for (int j = 0; j < K; ++j) {
       unsigned long long top = 0;
-      auto see = [&](unsigned long long key) { if (key < last && key > top) top = key; };
-      if (tid < K) see(ended(tid));
-      for (int e = tid; e < total; e += 64 * JW) see(entry(e));
+      each([&](unsigned long long key) { if (key < last && key > top) top = key; });
       top = max64(top);
       if (lane == 0) red[wave] = top;
       __syncthreads();
@@ -323,7 +363,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     {
       const int kc = base + tid;       // (beam, chunk); one that starts behind the last winner cannot hold a lower index
       if (kc < K * l.chunks && (unsigned)(entry(kc * K + K - 1) >> 32) == edge &&
-          ((unsigned)(kc / l.chunks) << 20 | (unsigned)(kc % l.chunks) * l.tiles * TILE) < beam_key_index(won[K - 1]))
+          ((unsigned)(kc / l.chunks) << 20 | (unsigned)(kc % l.chunks) * l.tiles * l.tile) < beam_key_index(won[K - 1]))
         again[atomicAdd(&have, 1)] = kc;
     }
     __syncthreads();
@@ -332,12 +372,12 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
       const int k = again[i] / l.chunks, c = again[i] % l.chunks;
       const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row;
       const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row : nullptr;
-      const long v1 = min((long)V, (long)(c + 1) * l.tiles * TILE);
+      const long v1 = min((long)V, (long)(c + 1) * l.tiles * l.tile);
       // the symbols of the edge's score, lowest first, until one does not beat the last winner
       unsigned long long last = ~0ull;
       for (int round = 0; round < K; ++round) {
         unsigned long long top = 0;
-        for (long v = (long)c * l.tiles * TILE + tid; v < v1; v += 64 * JW) {
+        for (long v = (long)c * l.tiles * l.tile + tid; v < v1; v += 64 * JW) {
           if (mk && !mk[v]) continue;
           const float sc = beam_score(to_f32<T>(r[v]), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
           const unsigned long long key = beam_key(sc, (unsigned)k << 20 | (unsigned)v);
@@ -374,8 +414,9 @@ constexpr int SHORT_V = 128;
 // K best so far make the next tile cheap, and there are fewer lists to join.
 static BeamLong long_plan(int n, int K, int V) {
   BeamLong l = {};
-  const long tiles = (V + TILE - 1) / TILE, rows = (long)n * K;
-  l.tiles = (int)std::max<long>(1, std::min<long>(tiles, rows * tiles / 8192));
+  l.tile = V <= 512 ? 512 : 1024;
+  const long tiles = (V + l.tile - 1) / l.tile, rows = (long)n * K;
+  l.tiles = (int)std::max<long>(1, std::min<long>(tiles, rows * tiles / 4096));
   l.chunks = (int)((tiles + l.tiles - 1) / l.tiles);
   return l;
 }
@@ -407,7 +448,9 @@ template <typename T> static int beam_select_t(const BeamSelect& a, void* ws, si
   PG_REQUIRE(lists < (1L << 26), "pg_beam_select: n=%d, K=%d, V=%d are too many rows for one call", a.n, a.K, a.V);
   l.part = at<BeamChunk>(ws, 0);
   l.keys = at<unsigned long long>(ws, align_up((size_t)lists * sizeof(BeamChunk), 256));
-  hipLaunchKernelGGL(beam_chunk_kernel<T>, dim3(cdiv(lists, SW)), dim3(64 * SW), 0, st, a, l);
+  const dim3 grid(cdiv(lists, SW)), block(64 * SW);
+  if (l.tile == 512) hipLaunchKernelGGL((beam_chunk_kernel<T, 8>), grid, block, 0, st, a, l);
+  else hipLaunchKernelGGL((beam_chunk_kernel<T, 16>), grid, block, 0, st, a, l);
   PG_CHECK_LAUNCH();
   hipLaunchKernelGGL(beam_join_kernel<T>, dim3(a.n), dim3(64 * JW), 0, st, a, l);
   PG_CHECK_LAUNCH();
