@@ -213,6 +213,18 @@ PG_API int pg_beam_select(int dtype, const void* logits, long ld_group, long ld_
                           int pad, int keep_slots, float* scores_out, int32_t* parents, int32_t* tokens, uint8_t* finished_out,
                           void* ws, size_t ws_bytes, void* stream);
 
+/* pg_beam_search: the K most probable strings of each of n latents by beam search over the decoder pg_sample samples from, with
+ * the steps of pg_beam_select (keep_slots) and the page moves below: a hypothesis' score is the sum of its log-probabilities
+ * under softmax(y / temp), and one that reached its eos competes with its score unchanged.  allowed (nullable): V bytes, 0 = the
+ * symbol is never taken.  tokens uint8 [n, K, max_len] best first (bos, symbols, eos, pad), end_pads int32 [n, K] as pg_sample's
+ * (max_len without an eos; 0 where there are fewer than K hypotheses), scores float [n, K] (-inf there).  max_len >= 2,
+ * K <= PG_MAX_BEAMS, n * K < 2^24; about 23 KB of workspace a beam (bf16 default decoder).  Molecules whose beams have all ended
+ * leave the decode.  Per-step kernels only: no persistent launch. */
+PG_API size_t pg_beam_search_workspace_bytes(const pg_dims* d, int dtype, int n, int K, int max_len);
+PG_API int pg_beam_search(const pg_dims* d, int dtype, const float* params, const void* shadow, void* ws, size_t ws_bytes, int n,
+                          int K, int max_len, const float* z, const uint8_t* allowed, double temp, uint8_t* tokens,
+                          int32_t* end_pads, float* scores, void* stream);
+
 /* Pages of a cache of decoder states.  A cache is n_planes arrays ("planes", e.g. the fp32 state and the operand copy of every
  * layer); page p is row p of every plane: `bytes` bytes at base + p * pitch.  Any width, pitch and alignment is taken; planes
  * of one call may interleave in one buffer but not share bytes (refused).  Indices live on the device and are checked by the

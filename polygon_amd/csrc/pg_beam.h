@@ -3,6 +3,15 @@
 #include "pg_common.h"
 #include "../../include/polygon_hip.h"
 
+// What a running search adds to a step (pg_beam_search.hip).  Groups are positions of a dense prefix that shrinks; scores,
+// finished flags and the history stay with the molecule.
+struct BeamTrack {
+  const int *n_dev, *mol;            // live positions; molecule at each
+  uint8_t *parent, *token;           // this step's history, [molecules, K]
+  uint8_t* live;                     // per position: some beam goes on
+  int* last;                         // per molecule: steps recorded
+  int step;
+};
 struct BeamSelect {
   const void* logits;
   long ld_group, ld_row;
@@ -264,8 +273,9 @@ __device__ __forceinline__ void beam_best(const float (&c)[N], F index, float be
 // One wave; won[] holds the group's K keys by rank, fin the finished beams as bits.
 // keep: the best child of a beam takes the beam's place (won[] is by rank, so it is the lowest lane that names the parent),
 // the others take the free places in ascending order, then come the entries without a candidate.  place[]: room for K.
-__device__ __forceinline__ void beam_write(const BeamSelect& a, long g, const unsigned long long* won, unsigned fin, int* place,
-                                           int lane) {
+template <bool TRACK>
+__device__ __forceinline__ void beam_write(const BeamSelect& a, const BeamTrack& tr, long g, long mol, const unsigned long long* won,
+                                           unsigned fin, int* place, int lane) {
   const int K = a.K;
   const unsigned long long key = lane < K ? won[lane] : 0;
   const unsigned index = beam_key_index(key);
@@ -287,10 +297,19 @@ __device__ __forceinline__ void beam_write(const BeamSelect& a, long g, const un
     const unsigned long long rest = __ballot(lane < K && !is_first);
     if (lane < K) to = is_first ? parent : place[lanes_before(rest)];
   }
+  const bool done = lane < K && (!key || (fin >> parent & 1) || v == a.eos);
+  if (TRACK) {
+    const bool goes_on = __ballot(lane < K && !done) != 0;
+    if (lane == 0) { tr.live[g] = goes_on; tr.last[mol] = tr.step; }
+  }
   if (lane >= K) return;
-  const long o = g * K + to;
-  a.scores_out[o] = key ? beam_key_number(key) : -INFINITY;
+  const long o = g * K + to, om = mol * K + to;      // (mol == g outside a search)
+  a.scores_out[om] = key ? beam_key_number(key) : -INFINITY;
+  a.finished_out[om] = done;
   a.parents[o] = key ? parent : to;
   a.tokens[o] = v;
-  a.finished_out[o] = !key || (fin >> parent & 1) || v == a.eos;
+  if (TRACK) { tr.parent[om] = key ? parent : to; tr.token[om] = v; }
 }
+
+// One step of a search over short vocabularies (V <= 128): logits fp32 [positions, K, ld].
+int launch_beam_track(const BeamSelect& a, const BeamTrack& tr, hipStream_t st);

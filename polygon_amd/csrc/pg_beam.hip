@@ -9,21 +9,23 @@
 // of them), all of softmax's reductions are inside 16 lanes (DPP).  With G > 1 the first wave selects from the G waves' best.
 // Bound by instructions: about half of them the selection, a quarter the 64-bit exponentials.
 constexpr int SW = 4;      // waves per workgroup
-template <typename T, int E, int P, int G>
-__global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a) {
+template <typename T, int E, int P, int G, bool TRACK>
+__global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a, BeamTrack tr) {
   __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
   __shared__ double sum_s[SW][4 * P];
   __shared__ int place_s[SW][PG_MAX_BEAMS];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const long g = ((long)blockIdx.x * SW + wave) / G;
-  if (G == 1 && g >= a.n) return;             // (G > 1: such a wave has no open beam, and takes part in the barrier)
+  const int n = TRACK ? min(a.n, *tr.n_dev) : a.n;
+  if (G == 1 && g >= n) return;               // (G > 1: such a wave has no open beam, and takes part in the barrier)
+  const long mol = TRACK && g < n ? tr.mol[g] : g;
   const int K = a.K, V = a.V, k0 = wave % G * (4 * P), row = lane >> 4;
   // beam `lane`
   float s_mine = -INFINITY;
   bool fin_mine = false;
-  if (lane < K && (G == 1 || g < a.n)) {
-    s_mine = a.scores[g * K + lane];
-    fin_mine = a.finished && a.finished[g * K + lane];
+  if (lane < K && (G == 1 || g < n)) {
+    s_mine = a.scores[mol * K + lane];
+    fin_mine = a.finished && a.finished[mol * K + lane];
   }
   const unsigned fin = (unsigned)__ballot(fin_mine), alive = (unsigned)__ballot(isfinite(s_mine)), open = alive & ~fin;
   // the lane's symbols v0 .. v0+E-1 of its rows; the row's last lane reads the last E, and leaves out those it shares
@@ -88,7 +90,7 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
                    list_s[wave], 0, won_s[wave], lane);
   if (G > 1) {
     __syncthreads();
-    if (wave % G != 0 || g >= a.n) return;
+    if (wave % G != 0 || g >= n) return;
     float t[G], top = -INFINITY;
     unsigned at[G];
 #pragma unroll
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
     }
     beam_best<G>(t, [&](int i) { return at[i]; }, top, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
   }
-  beam_write(a, g, won_s[wave], fin, place_s[wave], lane);
+  beam_write<TRACK>(a, tr, g, mol, won_s[wave], fin, place_s[wave], lane);
 }
 
 // ---- long vocabularies ------------------------------------------------------------------------------------------------
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   // that score.  It takes all of a group's winners coming from one chunk.
   const unsigned edge = (unsigned)(won[K - 1] >> 32);
   if (edge == 0) {
-    if (wave == 0) beam_write(a, g, won, fin, place, lane);
+    if (wave == 0) beam_write<false>(a, BeamTrack{}, g, g, won, fin, place, lane);
     return;
   }
   for (int base = 0; base < K * l.chunks; base += 64 * JW) {
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     }
     __syncthreads();
   }
-  if (wave == 0) beam_write(a, g, won, fin, place, lane);
+  if (wave == 0) beam_write<false>(a, BeamTrack{}, g, g, won, fin, place, lane);
 }
 
 constexpr int SHORT_V = 128;
@@ -429,18 +431,23 @@ extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V)
   return align_up(lists * sizeof(BeamChunk), 256) + lists * K * 8;
 }
 
+template <typename T, bool TRACK> static int launch_short(const BeamSelect& a, const BeamTrack& tr, hipStream_t st) {
+  auto go = [&](auto kernel, int G) { hipLaunchKernelGGL(kernel, dim3(cdiv((long)a.n * G, SW)), dim3(64 * SW), 0, st, a, tr); };
+  const bool narrow = a.V <= 64;
+  if (a.K <= 4) narrow ? go(beam_select_short_kernel<T, 4, 1, 1, TRACK>, 1) : go(beam_select_short_kernel<T, 8, 1, 1, TRACK>, 1);
+  else if (a.K <= 8) narrow ? go(beam_select_short_kernel<T, 4, 2, 1, TRACK>, 1) : go(beam_select_short_kernel<T, 8, 2, 1, TRACK>, 1);
+  else if (a.K <= 16) narrow ? go(beam_select_short_kernel<T, 4, 2, 2, TRACK>, 2) : go(beam_select_short_kernel<T, 8, 2, 2, TRACK>, 2);
+  else narrow ? go(beam_select_short_kernel<T, 4, 2, 4, TRACK>, 4) : go(beam_select_short_kernel<T, 8, 2, 4, TRACK>, 4);
+  PG_CHECK_LAUNCH();
+  return PG_OK;
+}
+int launch_beam_track(const BeamSelect& a, const BeamTrack& tr, hipStream_t st) {
+  PG_REQUIRE(a.V <= SHORT_V && a.K <= PG_MAX_BEAMS, "beam search: V=%d or K=%d out of range", a.V, a.K);
+  return launch_short<float, true>(a, tr, st);
+}
+
 template <typename T> static int beam_select_t(const BeamSelect& a, void* ws, size_t ws_bytes, hipStream_t st) {
-  if (a.V <= SHORT_V) {
-#define PG_SHORT(E, P, G) hipLaunchKernelGGL((beam_select_short_kernel<T, E, P, G>), dim3(cdiv((long)a.n * G, SW)), dim3(64 * SW), 0, st, a)
-#define PG_SHORT_E(E) \
-  do { if (a.K <= 4) PG_SHORT(E, 1, 1); else if (a.K <= 8) PG_SHORT(E, 2, 1); else if (a.K <= 16) PG_SHORT(E, 2, 2); else PG_SHORT(E, 2, 4); } while (0)
-    if (a.V <= 64) PG_SHORT_E(4);
-    else PG_SHORT_E(8);
-#undef PG_SHORT_E
-#undef PG_SHORT
-    PG_CHECK_LAUNCH();
-    return PG_OK;
-  }
+  if (a.V <= SHORT_V) return launch_short<T, false>(a, BeamTrack{}, st);
   const size_t need = pg_beam_select_workspace_bytes(0, a.n, a.K, a.V);
   if (!ws || ws_bytes < need) PG_FAIL(PG_ERR_WORKSPACE, "pg_beam_select: workspace too small (%zu < %zu)", ws_bytes, need);
   BeamLong l = long_plan(a.n, a.K, a.V);

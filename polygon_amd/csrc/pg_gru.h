@@ -7,6 +7,8 @@ enum { PG_GI_ARRAY = 0, PG_GI_TABLE = 1, PG_GI_FUSED = 2, PG_GI_DYN = 3 /* kerne
 
 template <typename T> struct GruFwdArgs {
   int rows = 0, H = 0;
+  const int* groups_dev = nullptr;  // optional: only the first *groups_dev * group_rows rows are live (known on the device only)
+  int group_rows = 1;               // neighbouring rows that share a row of zproj (TABLE); with groups_dev, the unit it counts
   // recurrent operand h_{t-1}: operand-dtype copy feeds the MFMA, fp32 copy feeds z*h_prev.  Both null => h_prev = 0.
   const T* hprev_op = nullptr;
   const float* hprev32 = nullptr;
@@ -17,7 +19,7 @@ template <typename T> struct GruFwdArgs {
   const float* gi = nullptr;   // ARRAY: [rows, 3H]
   const float* table = nullptr; // TABLE: [V, 3H] rows gathered by tok[]
   const int* tok = nullptr;     // TABLE: [rows]
-  const float* zproj = nullptr; // TABLE: optional [rows, 3H] added per row (decoder layer 0: W_ih[:, E:] z)
+  const float* zproj = nullptr; // TABLE: optional [rows / group_rows, 3H] added per row (decoder layer 0: W_ih[:, E:] z)
   const T* x = nullptr;         // FUSED: [rows, Kx]
   int Kx = 0;
   const T* Wih = nullptr;       // FUSED: [3H, Kx]

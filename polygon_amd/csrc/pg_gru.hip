@@ -276,7 +276,7 @@ __device__ __forceinline__ void gru_fwd2_body(const GruFwdArgs<T>& a, int bx, in
         Vec8<float>::load(g, gr[c]); Vec8<float>::load(g + H, gz[c]); Vec8<float>::load(g + 2 * H, gn[c]);
         if (a.zproj) {
           float t0[8], t1[8], t2[8];
-          const float* zp = a.zproj + (long)b * 3 * H + j;
+          const float* zp = a.zproj + (long)(a.group_rows > 1 ? b / a.group_rows : b) * 3 * H + j;
           Vec8<float>::load(zp, t0); Vec8<float>::load(zp + H, t1); Vec8<float>::load(zp + 2 * H, t2);
 #pragma unroll
           for (int i = 0; i < 8; ++i) { gr[c][i] += t0[i]; gz[c][i] += t1[i]; gn[c][i] += t2[i]; }
@@ -359,6 +359,10 @@ __device__ __forceinline__ void gru_fwd2_body(const GruFwdArgs<T>& a, int bx, in
 template <typename T, int MODE, int G, int D>
 __global__ __launch_bounds__(256 * G) void gru_fwd2_kernel(GruFwdArgs<T> a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if (a.groups_dev) {   // uniform over the launch
+    a.rows = min(a.rows, *a.groups_dev * a.group_rows);
+    if ((int)blockIdx.y * V2_BM >= a.rows) return;
+  }
   gru_fwd2_body<T, MODE, G, D>(a, blockIdx.x, blockIdx.y, smem);
 }
 template <typename T, int G, int D>
@@ -527,7 +531,8 @@ template <typename T> int launch_gru_fwd(const GruFwdArgs<T>& a, hipStream_t str
   PG_REQUIRE(a.H % EPC == 0 && a.H >= 32, "gru_fwd: hidden size %d must be a multiple of %d", a.H, EPC);
   PG_REQUIRE(a.gi_mode != PG_GI_FUSED || (a.Kx % EPC == 0), "gru_fwd: fused input width %d must be a multiple of %d", a.Kx, EPC);
   PG_REQUIRE((a.hprev_op == nullptr) == (a.hprev32 == nullptr), "gru_fwd: hprev_op / hprev32 must both be set or null");
-  static const int variant = getenv("PG_FWD_VARIANT") ? atoi(getenv("PG_FWD_VARIANT")) : 0;   // tuning aid
+  static const int variant_env = getenv("PG_FWD_VARIANT") ? atoi(getenv("PG_FWD_VARIANT")) : 0;   // tuning aid
+  const int variant = a.group_rows > 1 && variant_env > 2 ? 0 : variant_env;   // (3, 4: kernels without the grouped rows)
   if (variant == 1 || variant == 2) {
     if (variant == 1) {
       if (a.gi_mode == PG_GI_ARRAY) return launch_fwd2<PG_GI_ARRAY, 1, 2, T>(a, stream);

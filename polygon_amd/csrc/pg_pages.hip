@@ -1,6 +1,6 @@
 // Pages of a cache of decoder states: reorder inside groups, fork, compaction.
+#include "pg_pages.h"
 #include "pg_host.h"
-#include "../../include/polygon_hip.h"
 
 // What a move kernel needs of a cache: its planes, and where each plane's first column segment is counted.  A segment is
 // PG_SEG bytes of a page: 16 bytes for each lane of a wave.
@@ -77,9 +77,10 @@ __device__ __forceinline__ int seg_plane(const Planes& pl, int seg) {
 // Bound by HBM: 16 bytes per lane, up to R loads in flight per wave.
 template <int R, bool REORDER>
 __global__ __launch_bounds__(256) void pages_move_kernel(Planes dst, Planes src, long units, int K, long n_dst, unsigned n_src,
-                                                         const int32_t* __restrict__ from) {
+                                                         const int32_t* __restrict__ from, const int* __restrict__ groups_dev) {
   const int lane = threadIdx.x & 63;
   const int segs = dst.first[dst.n];
+  if (groups_dev) units = min(units, (long)*groups_dev * segs);
   for (long u = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (long)gridDim.x * 4) {
     const long g = u / segs;
     const int seg = (int)(u - g * segs), i = seg_plane(dst, seg);
@@ -179,8 +180,10 @@ static int compact_grid(long n, long segs) { return (int)std::max<long>(1, std::
 // Up to PLAN_PAGES pages: ONE launch, every workgroup works the plan out for itself (n flag bytes from L2, a scan, the moves'
 // ends as 16-bit lists in LDS) and takes its share of the moves.
 constexpr int PLAN_PAGES = 16384;
-__global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, const uint8_t* __restrict__ live,
-                                                            int32_t* __restrict__ count, int32_t* __restrict__ map) {
+__global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, const int* __restrict__ n_dev,
+                                                            const uint8_t* __restrict__ live, int32_t* __restrict__ count,
+                                                            int32_t* __restrict__ map) {
+  if (n_dev) n = min(n, *n_dev);
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ unsigned long long bits[256];
   __shared__ int before[256], part[4], low_s;
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, co
   }
   __syncthreads();
   if (blockIdx.x == 0 && tid == 0) count[0] = total;
-  for (int p = blockIdx.x * 256 + tid; p < n; p += gridDim.x * 256) {
+  for (int p = blockIdx.x * 256 + tid; map && p < n; p += gridDim.x * 256) {
     const int t = p / per, i = p % per;
     const bool l = bits[t] >> i & 1;
     map[p] = !l ? -1 : p < total ? p : (int)hole[before[t] + __popcll(bits[t] & ((1ull << i) - 1)) - low];
@@ -221,9 +224,11 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, co
 }
 
 // More pages: the plan by one workgroup into the workspace, then the moves.
-__global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const uint8_t* __restrict__ live, int32_t* __restrict__ count,
+__global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const int* __restrict__ n_dev,
+                                                          const uint8_t* __restrict__ live, int32_t* __restrict__ count,
                                                           int32_t* __restrict__ map, int32_t* __restrict__ moves,
                                                           int32_t* __restrict__ hole, int32_t* __restrict__ mover) {
+  if (n_dev) n = min(n, *n_dev);
   __shared__ int part[16], part2[16];
   const int tid = threadIdx.x;
   const long per = ((n + 1023L) / 1024 + 7) / 8 * 8, p0 = min((long)n, tid * per), p1 = min((long)n, p0 + per);
@@ -242,36 +247,43 @@ __global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const uint8_t* 
       const long q = p + i;
       if (q < total) {
         if (!l) hole[q - before] = (int)q;
-        map[q] = l ? (int)q : -1;
+        if (map) map[q] = l ? (int)q : -1;
       } else if (l) mover[before - low] = (int)q;
-      else map[q] = -1;
+      else if (map) map[q] = -1;
       before += l;
     }
   }
   __syncthreads();
-  for (int i = tid; i < total - low; i += 1024) map[mover[i]] = hole[i];
+  if (map)
+    for (int i = tid; i < total - low; i += 1024) map[mover[i]] = hole[i];
 }
 __global__ __launch_bounds__(256) void pages_compact_move_kernel(Planes pl, const int32_t* __restrict__ moves,
                                                                  const int32_t* __restrict__ hole, const int32_t* __restrict__ mover) {
   move_pages(pl, moves[0], hole, mover);
 }
 
+int launch_pages_reorder(const pg_plane* planes, int n_planes, int n_groups, const int* groups_dev, int K, const int32_t* parents,
+                         hipStream_t st) {
+  Planes pl;
+  PG_TRY(make_planes("pg_pages_reorder", planes, n_planes, &pl));
+  const long units = (long)n_groups * pl.first[n_planes], pages = (long)n_groups * K;
+  // R registers of 16 bytes per lane: the narrowest instantiation that holds the group
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents, groups_dev);
+  };
+  if (K <= 8) go(pages_move_kernel<8, true>);
+  else if (K <= 16) go(pages_move_kernel<16, true>);
+  else go(pages_move_kernel<32, true>);
+  PG_CHECK_LAUNCH();
+  return PG_OK;
+}
 extern "C" int pg_pages_reorder(const pg_plane* planes, int n_planes, int n_groups, int K, const int32_t* parents, void* stream) {
   PG_REQUIRE(n_groups >= 0 && K >= 1 && K <= PG_MAX_BEAMS, "pg_pages_reorder: n_groups=%d or K=%d outside [1,%d]", n_groups, K,
              PG_MAX_BEAMS);
   PG_TRY(check_planes("pg_pages_reorder", planes, n_planes, (long)n_groups * K));
   if (n_groups == 0) return PG_OK;
   PG_REQUIRE(parents, "pg_pages_reorder: parents is NULL");
-  Planes pl;
-  PG_TRY(make_planes("pg_pages_reorder", planes, n_planes, &pl));
-  const long units = (long)n_groups * pl.first[n_planes], pages = (long)n_groups * K;
-  const hipStream_t st = (hipStream_t)stream;
-  // R registers of 16 bytes per lane: the narrowest instantiation that holds the group
-  if (K <= 8) hipLaunchKernelGGL((pages_move_kernel<8, true>), dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents);
-  else if (K <= 16) hipLaunchKernelGGL((pages_move_kernel<16, true>), dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents);
-  else hipLaunchKernelGGL((pages_move_kernel<32, true>), dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents);
-  PG_CHECK_LAUNCH();
-  return PG_OK;
+  return launch_pages_reorder(planes, n_planes, n_groups, nullptr, K, parents, (hipStream_t)stream);
 }
 
 extern "C" int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_planes, int n_dst, int n_src, const int32_t* index,
@@ -294,7 +306,7 @@ extern "C" int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_pla
   constexpr int R = 8;
   const long units = (long)cdiv(n_dst, R) * d.first[n_planes];
   hipLaunchKernelGGL((pages_move_kernel<R, false>), dim3(move_grid(units)), dim3(256), 0, (hipStream_t)stream, d, s, units, R, (long)n_dst,
-                     (unsigned)n_src, index);
+                     (unsigned)n_src, index, (const int*)nullptr);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
@@ -305,6 +317,23 @@ extern "C" size_t pg_pages_compact_workspace_bytes(int n_pages) {
   return n_pages <= PLAN_PAGES ? 0 : 256 + 2 * compact_list_bytes(n_pages);
 }
 
+int launch_pages_compact(const pg_plane* planes, int n_planes, int n_pages, const int* n_dev, const uint8_t* live, int32_t* count,
+                         int32_t* map, void* ws, hipStream_t st) {
+  Planes pl;
+  PG_TRY(make_planes("pg_pages_compact", planes, n_planes, &pl));
+  const int grid = compact_grid(n_pages, pl.first[n_planes]);
+  if (n_pages <= PLAN_PAGES) {
+    hipLaunchKernelGGL(pages_compact_kernel, dim3(grid), dim3(256), (size_t)(n_pages / 2) * 4, st, pl, n_pages, n_dev, live, count, map);
+    PG_CHECK_LAUNCH();
+    return PG_OK;
+  }
+  int32_t *moves = at<int32_t>(ws, 0), *hole = at<int32_t>(ws, 256), *mover = at<int32_t>(ws, 256 + compact_list_bytes(n_pages));
+  hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(1024), 0, st, n_pages, n_dev, live, count, map, moves, hole, mover);
+  PG_CHECK_LAUNCH();
+  hipLaunchKernelGGL(pages_compact_move_kernel, dim3(grid), dim3(256), 0, st, pl, moves, hole, mover);
+  PG_CHECK_LAUNCH();
+  return PG_OK;
+}
 extern "C" int pg_pages_compact(const pg_plane* planes, int n_planes, int n_pages, const uint8_t* live, int32_t* count, int32_t* map,
                                 void* ws, size_t ws_bytes, void* stream) {
   PG_REQUIRE(n_pages >= 0, "pg_pages_compact: n_pages=%d", n_pages);
@@ -312,19 +341,5 @@ extern "C" int pg_pages_compact(const pg_plane* planes, int n_planes, int n_page
   PG_REQUIRE(count && (n_pages == 0 || (live && map)), "pg_pages_compact: NULL buffer");
   const size_t need = pg_pages_compact_workspace_bytes(n_pages);
   if (ws_bytes < need || (need && !ws)) PG_FAIL(PG_ERR_WORKSPACE, "pg_pages_compact: workspace too small (%zu < %zu)", ws_bytes, need);
-  Planes pl;
-  PG_TRY(make_planes("pg_pages_compact", planes, n_planes, &pl));
-  const hipStream_t st = (hipStream_t)stream;
-  const int grid = compact_grid(n_pages, pl.first[n_planes]);
-  if (n_pages <= PLAN_PAGES) {
-    hipLaunchKernelGGL(pages_compact_kernel, dim3(grid), dim3(256), (size_t)(n_pages / 2) * 4, st, pl, n_pages, live, count, map);
-    PG_CHECK_LAUNCH();
-    return PG_OK;
-  }
-  int32_t *moves = at<int32_t>(ws, 0), *hole = at<int32_t>(ws, 256), *mover = at<int32_t>(ws, 256 + compact_list_bytes(n_pages));
-  hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(1024), 0, st, n_pages, live, count, map, moves, hole, mover);
-  PG_CHECK_LAUNCH();
-  hipLaunchKernelGGL(pages_compact_move_kernel, dim3(grid), dim3(256), 0, st, pl, moves, hole, mover);
-  PG_CHECK_LAUNCH();
-  return PG_OK;
+  return launch_pages_compact(planes, n_planes, n_pages, nullptr, live, count, map, ws, (hipStream_t)stream);
 }

@@ -19,6 +19,7 @@ import torch.nn as nn
 from polygon_amd import _lib
 from polygon_amd.utils.moses_utils import OneHotVocab
 from polygon_amd.utils.smiles_char_dict import SmilesCharDictionary
+from polygon_amd.vae.beam import MAX_BEAMS
 
 
 def get_vocabulary(data=None, device=None):
@@ -664,8 +665,13 @@ class VAE(nn.Module):
         z, kl_loss, mu = self.forward_encoder(x, return_mu=True)
         return mu
 
-    def decode(self, z, x=None):
-        """vae_model.py:183-200."""
+    def decode(self, z, x=None, beam_width=None):
+        """vae_model.py:183-200.  ``beam_width`` (no counterpart there): the most probable strings by beam search instead of drawn
+        ones (only without ``x``)."""
+        if beam_width is not None:
+            if x is not None:
+                raise ValueError("decode: beam_width is for decoding without teacher forcing (x=None)")
+            return [best[0] for best in self.beam_search(z, beam_width=beam_width)[0]]
         if x is not None:
             rl, y = self.forward_decoder(x, z, return_y=True)
             xr = y.argmax(2)
@@ -774,6 +780,52 @@ class VAE(nn.Module):
         """vae_model.py:300-358 -> list of strings (no early exit; specials mid-stream rendered literally)."""
         tokens, end_pads = self.sample_tokens(n_batch, max_len=max_len, z=z, temp=temp, multinomial=multinomial)
         return self.vocabulary.decode_batch(tokens.cpu().numpy(), end_pads.cpu().numpy())
+
+    def beam_search_tokens(self, z, beam_width=8, max_len=100, temp=1.0, allowed=None):
+        """Token form of ``beam_search``: (tokens uint8 [n, K, max_len], end_pads int32 [n, K], scores float32 [n, K]) on the
+        device, best hypothesis first.  Nothing is copied to the host or waited for."""
+        eng = self._engine
+        K = int(beam_width)
+        if z.dim() != 2 or z.shape[1] != self.d_z:
+            raise RuntimeError("z must be [n, %d], got %s" % (self.d_z, list(z.shape)))
+        n, V = z.shape[0], len(self.vocabulary)
+        with torch.no_grad():
+            eng.ensure_shadow()
+            dev = eng.flat.device
+            z = z.to(dev, torch.float32).contiguous()
+            if allowed is not None:
+                if tuple(allowed.shape) != (V,):
+                    raise RuntimeError("allowed must have shape [%d]" % V)
+                allowed = (allowed != 0).to(dev, torch.uint8).contiguous()
+            if not 1 <= K <= MAX_BEAMS:
+                raise RuntimeError("beam_width must lie in [1, %d], got %d" % (MAX_BEAMS, K))
+            L = _lib.lib()
+            L.pg_beam_search_workspace_bytes.restype = ctypes.c_size_t
+            tokens = torch.empty(n, K, max_len, dtype=torch.uint8, device=dev)
+            end_pads = torch.empty(n, K, dtype=torch.int32, device=dev)
+            scores = torch.empty(n, K, device=dev)
+            CH = max(1, 65536 // K)      # latents per library call: bounds the workspace (~23 KB per beam) whatever n is
+            for r0 in range(0, n, CH):
+                m = min(CH, n - r0)
+                nbytes = L.pg_beam_search_workspace_bytes(ctypes.byref(eng.dims), eng.dtype_code(), m, K, int(max_len))
+                if nbytes == 0:
+                    raise _lib.PolygonHipError("pg_beam_search_workspace_bytes: " + L.pg_last_error().decode())
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+                _lib.check(L.pg_beam_search(ctypes.byref(eng.dims), eng.dtype_code(), _lib.ptr(eng.flat), _lib.ptr(eng.shadow),
+                                            _lib.ptr(ws), ctypes.c_size_t(nbytes), m, K, int(max_len), _lib.ptr(z[r0:r0 + m]),
+                                            _lib.ptr(allowed), ctypes.c_double(float(temp)), _lib.ptr(tokens[r0:r0 + m]),
+                                            _lib.ptr(end_pads[r0:r0 + m]), _lib.ptr(scores[r0:r0 + m]), _lib.stream_ptr()),
+                           "pg_beam_search")
+            return tokens, end_pads, scores
+
+    def beam_search(self, z, beam_width=8, max_len=100, temp=1.0, allowed=None):
+        """The ``beam_width`` most probable strings of every latent z [n, d_z], best first (no counterpart in the reference, which
+        draws or takes the argmax symbol by symbol): (n lists of strings, scores float32 [n, beam_width] on the host: sums of
+        log-probabilities, -inf and '' where there are fewer hypotheses).  ``allowed`` [V] bool: symbols that may be taken."""
+        tokens, end_pads, scores = self.beam_search_tokens(z, beam_width, max_len, temp, allowed)
+        n, K = scores.shape
+        flat = self.vocabulary.decode_batch(tokens.flatten(0, 1).cpu().numpy(), end_pads.flatten().cpu().numpy())
+        return [flat[i * K:(i + 1) * K] for i in range(n)], scores.cpu()
 
     def sample_sharded(self, n_batch, max_len=100, temp=1.0, multinomial=True, seed=None, group=None):
         """``sample`` over the ranks of a torch.distributed job (no counterpart in the reference): the rows
