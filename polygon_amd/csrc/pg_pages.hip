@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, co
   __shared__ unsigned long long bits[256];
   __shared__ int before[256], part[4], low_s;
   const int tid = threadIdx.x;
-  const int per = n <= 2048 ? 8 : 64;                       // flags per thread (n <= 256 * per)
+  const int per = n <= 2048 ? 8 : n <= 4096 ? 16 : n <= 8192 ? 32 : 64;      // flags per thread (n <= 256 * per)
   unsigned long long mine = 0;
   for (int i = 0; i < per && (long)tid * per + i < n; i += 8) mine |= (unsigned long long)live_bits8(live, (long)tid * per + i, n) << i;
   int total;
@@ -203,9 +203,9 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, co
   const int low = low_s, moves = total - low;
   unsigned short *hole = reinterpret_cast<unsigned short*>(smem), *mover = hole + n / 2;
   const unsigned long long below = end >= 64 ? ~0ull : end > 0 ? (1ull << end) - 1 : 0;
-  const unsigned long long own = n - tid * per >= 64 ? ~0ull : n > tid * per ? (1ull << (n - tid * per)) - 1 : 0;
-  const unsigned long long lane_own = per == 64 ? own : own & 0xFFull;
-  for (unsigned long long h = ~mine & below & lane_own; h; h &= h - 1) {
+  const int own_n = min(per, n - tid * per);                // my flags
+  const unsigned long long own = own_n >= 64 ? ~0ull : own_n > 0 ? (1ull << own_n) - 1 : 0;
+  for (unsigned long long h = ~mine & below & own; h; h &= h - 1) {
     const int i = __ffsll(h) - 1;
     hole[tid * per + i - (b + __popcll(mine & ((1ull << i) - 1)))] = (unsigned short)(tid * per + i);
   }

@@ -7,6 +7,7 @@ checked on the host (shapes, types, devices, strides); indices are device data a
 range moves nothing.  Nothing here is differentiable.
 """
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -14,6 +15,7 @@ import torch
 from polygon_amd import _lib
 
 MAX_BEAMS = 32      # PG_MAX_BEAMS
+NO_WORKSPACE_V = 128      # up to here pg_beam_select_workspace_bytes is 0: not asked
 
 
 class BeamStep(NamedTuple):
@@ -53,14 +55,14 @@ def _call(device, entry, *args):
     else:
         with torch.cuda.device(at):
             status = entry(*args, torch._C._cuda_getCurrentRawStream(at))
-    if status != 0:
+    if status:
         _lib.check(status, entry.__name__)
 
 
 def _flags(t, shape, device, what):
-    if t.dtype not in (torch.bool, torch.uint8):
+    if t.dtype is not torch.bool and t.dtype is not torch.uint8:
         raise ValueError("%s must be bool or uint8, got %s" % (what, t.dtype))
-    if tuple(t.shape) != tuple(shape) or t.device != device:
+    if t.shape != shape or t.device != device:
         raise ValueError("%s must be %s on %s, got %s on %s" % (what, list(shape), device, list(t.shape), t.device))
     return t.contiguous()
 
@@ -80,7 +82,7 @@ def beam_select(logits, scores, finished=None, mask=None, temp=1.0, eos=-1, pad=
         raise ValueError("logits must be [n, K, V] float32 or bfloat16, got %s %s" % (list(logits.shape), logits.dtype))
     n, K, V = logits.shape
     dev = logits.device
-    if tuple(scores.shape) != (n, K) or scores.dtype != torch.float32 or scores.device != dev:
+    if scores.shape != (n, K) or scores.dtype != torch.float32 or scores.device != dev:
         raise ValueError("scores must be [%d, %d] float32 on %s, got %s %s on %s" % (n, K, dev, list(scores.shape), scores.dtype,
                                                                                   scores.device))
     if V > 1 and logits.stride(2) != 1:
@@ -102,35 +104,39 @@ def beam_select(logits, scores, finished=None, mask=None, temp=1.0, eos=-1, pad=
         if mask.dim() > 2 and mask.shape[0] > 1:
             mg = mask.stride(0)
     L = _entries()
-    new = scores.new_empty
-    out = BeamStep(new((n, K)), new((n, K), dtype=torch.int32), new((n, K), dtype=torch.int32), new((n, K), dtype=torch.bool))
+    like = torch.empty_like              # (the quickest way to an output's memory)
+    parents = like(scores, dtype=torch.int32)
+    out = BeamStep(like(scores), parents, like(parents), like(scores, dtype=torch.bool))
     code = _lib.PG_F32 if logits.dtype == torch.float32 else _lib.PG_BF16
-    need = L.pg_beam_select_workspace_bytes(code, n, K, V)
-    ws = new(need, dtype=torch.uint8) if need else None
+    need = L.pg_beam_select_workspace_bytes(code, n, K, V) if V > NO_WORKSPACE_V else 0
+    ws = scores.new_empty(need, dtype=torch.uint8) if need else None
     _call(dev, L.pg_beam_select, code, logits.data_ptr(), logits.stride(0), logits.stride(1), n, K, V,
           None if mask is None else mask.data_ptr(), mg, mr, float(temp), scores.data_ptr(),
-          None if finished is None else finished.data_ptr(), int(eos), int(pad), int(bool(keep_slots)), out.scores.data_ptr(),
-          out.parents.data_ptr(), out.tokens.data_ptr(), out.finished.data_ptr(), None if ws is None else ws.data_ptr(), need)
+          None if finished is None else finished.data_ptr(), int(eos), int(pad), int(bool(keep_slots)),
+          *[t.data_ptr() for t in out], None if ws is None else ws.data_ptr(), need)
     return out
 
 
 def _planes(planes, what):
-    """The C description of a cache: its planes' first dimension counts pages, what is behind it is one page's dense row."""
+    """The C description of a cache (pg_plane: base, pitch, bytes - three words a plane): the planes' first dimension counts pages,
+    what is behind it is one page's dense row."""
     if not planes:
         raise ValueError("%s: no planes" % what)
-    dev, P = planes[0].device, planes[0].shape[0] if planes[0].dim() else -1
+    shape, dev = planes[0].shape, planes[0].device
+    P = shape[0] if shape else -1
     out = []
     for t in planes:
-        if t.dim() < 1 or t.shape[0] != P or t.device != dev:
+        shape = t.shape
+        if not shape or shape[0] != P or t.device != dev:
             raise ValueError("%s: every plane must have the same number of pages in front, on one device" % what)
         if t.requires_grad:
             raise ValueError("%s: pages are moved in place, a plane must not require gradients" % what)
-        size = t.element_size()
         if P and t.is_contiguous():
-            row = pitch = t.numel() // P * size
+            row = pitch = t.nbytes // P
         else:
-            row, pitch = size, t.stride(0) * size
-            for extent, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            row = size = t.element_size()
+            pitch = t.stride(0) * size
+            for extent, stride in zip(reversed(shape[1:]), reversed(t.stride()[1:])):
                 if extent != 1 and stride * size != row:
                     raise ValueError("%s: what is behind a plane's first dimension must be dense, got strides %s" % (what, list(t.stride())))
                 row *= extent
@@ -139,7 +145,7 @@ def _planes(planes, what):
         if row == 0:
             raise ValueError("%s: a page of no bytes" % what)
         out += (t.data_ptr(), pitch, row)
-    return (ctypes.c_long * len(out))(*out), dev, P
+    return struct.pack("%dQ" % len(out), *out), dev, P
 
 
 def _index(t, dev, what):
@@ -152,10 +158,11 @@ def reorder_pages(planes, parents):
     """In place: page g*K + j of every plane takes over what page g*K + parents[g, j] held before the call.  ``planes``:
     tensors [n*K, ...], dense behind the first dimension; ``parents`` [n, K] int32 (``BeamStep.parents``)."""
     d, dev, P = _planes(planes, "reorder_pages")
-    if parents.dim() != 2 or parents.shape[0] * parents.shape[1] != P:
-        raise ValueError("parents %s does not name %d pages" % (list(parents.shape), P))
+    shape = parents.shape
+    if len(shape) != 2 or shape[0] * shape[1] != P:
+        raise ValueError("parents %s does not name %d pages" % (list(shape), P))
     parents = _index(parents, dev, "parents")
-    _call(dev, _entries().pg_pages_reorder, d, len(planes), parents.shape[0], parents.shape[1], parents.data_ptr())
+    _call(dev, _entries().pg_pages_reorder, d, len(planes), shape[0], shape[1], parents.data_ptr())
 
 
 def fork_pages(dst, src, index):
