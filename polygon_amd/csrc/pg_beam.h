@@ -197,13 +197,13 @@ __device__ __forceinline__ void beam_rank(const unsigned long long* list, int m,
   wave_sync();
 }
 
-// The K best of a wave's N numbers per lane, those above `above` only (-inf: all), and of the `m` keys that list[] (room for
-// 128) already holds, into won[0 .. K) by rank (keys; 0 where there are fewer).  index(i): of a lane's i-th number.
-// best: the lane's largest number.  What reaches the bound is nearly always few; where it is not (ties all over) the keys are
-// taken out one by one.
+// Puts a few keys (at most 128 in all; the new length is returned) behind the `m` <= 64 that list[] already holds, the K best of
+// a wave's N numbers per lane among them; only numbers above `above` (-inf: all) count.  index(i): of a lane's i-th number.
+// best: the lane's largest number.  What reaches the bound is nearly always few; where it is not (ties all over) the K best of
+// everything are taken out one by one, by way of won[].
 template <int N, class F>
-__device__ __forceinline__ void beam_best(const float (&c)[N], F index, float best, float above, int K, unsigned long long* list, int m,
-                                          unsigned long long* won, int lane) {
+__device__ __forceinline__ int beam_collect(const float (&c)[N], F index, float best, float above, int K, unsigned long long* list, int m,
+                                            unsigned long long* won, int lane) {
   const int some = __popcll(__ballot(best > above));
   float bound = some > K ? beam_bound(best, above, K) : beam_unorder(beam_order(above) + 1);
   const int m0 = m;
@@ -222,11 +222,12 @@ __device__ __forceinline__ void beam_best(const float (&c)[N], F index, float be
     wave_sync();
   };
   put();
-  if (m > 128) {
+  const int limit = m0 + K + 24 > 64 ? 128 : 64;       // (a ranking of 64 costs as much as four steps here)
+  if (m > limit) {
     // a few lanes hold most of it (rows of very different scores): halve by numbers instead of lanes
     unsigned lo = beam_order(bound), hi = beam_order(max64(best)) + 1;
     int all = m - m0;
-    while (all + m0 > 128 && hi - lo > 1) {
+    while (all + m0 > limit && hi - lo > 1) {
       const unsigned mid = lo + (hi - lo) / 2;
       const float f = beam_unorder(mid);
       int n = 0;
@@ -238,10 +239,7 @@ __device__ __forceinline__ void beam_best(const float (&c)[N], F index, float be
     bound = beam_unorder(lo);
     if (all + m0 <= 128) put();
   }
-  if (m <= 128) {
-    beam_rank(list, m, won, K, lane);
-    return;
-  }
+  if (m <= 128) return m;
   // (rare: written so that it needs no registers of its own - `zero` keeps the indices from being worked out ahead of the loop)
   float last = INFINITY;
   unsigned last_i = 0;
@@ -267,6 +265,16 @@ __device__ __forceinline__ void beam_best(const float (&c)[N], F index, float be
     last_i = top_i;
   }
   wave_sync();
+  const unsigned long long key = lane < K ? won[lane] : 0;
+  if (lane < K) list[lane] = key;
+  wave_sync();
+  return __popcll(__ballot(key != 0));
+}
+// The same, ranked: the K best of both into won[0 .. K) (keys; 0 where there are fewer).
+template <int N, class F>
+__device__ __forceinline__ void beam_best(const float (&c)[N], F index, float best, float above, int K, unsigned long long* list, int m,
+                                          unsigned long long* won, int lane) {
+  beam_rank(list, beam_collect<N>(c, index, best, above, K, list, m, won, lane), won, K, lane);
 }
 
 // ---- the step's outputs -----------------------------------------------------------------------------------------------

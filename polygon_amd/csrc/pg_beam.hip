@@ -86,21 +86,25 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
       best = fmaxf(best, f);
     }
   }
-  beam_best<P * E>(c, [&](int i) { return (unsigned)(k0 + i / E * 4 + row) << 20 | (unsigned)(v0 + i % E); }, best, -INFINITY, K,
-                   list_s[wave], 0, won_s[wave], lane);
-  if (G > 1) {
+  auto index = [&](int i) { return (unsigned)(k0 + i / E * 4 + row) << 20 | (unsigned)(v0 + i % E); };
+  if (G == 1) beam_best<P * E>(c, index, best, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
+  else {   // every wave's few, unranked; the group's first wave selects from them
+    __shared__ int many_s[SW];
+    const int many = beam_collect<P * E>(c, index, best, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
+    if (lane == 0) many_s[wave] = many;
     __syncthreads();
     if (wave % G != 0 || g >= n) return;
-    float t[G], top = -INFINITY;
-    unsigned at[G];
+    float t[2 * G], top = -INFINITY;
+    unsigned at[2 * G];
 #pragma unroll
-    for (int w = 0; w < G; ++w) {
-      const unsigned long long key = lane < K ? won_s[wave + w][lane] : 0;
-      t[w] = key ? beam_key_number(key) : -INFINITY;
-      at[w] = beam_key_index(key);
-      top = fmaxf(top, t[w]);
+    for (int i = 0; i < 2 * G; ++i) {
+      const int j = lane + i % 2 * 64;
+      const unsigned long long key = j < many_s[wave + i / 2] ? list_s[wave + i / 2][j] : 0;
+      t[i] = key ? beam_key_number(key) : -INFINITY;
+      at[i] = beam_key_index(key);
+      top = fmaxf(top, t[i]);
     }
-    beam_best<G>(t, [&](int i) { return at[i]; }, top, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
+    beam_best<2 * G>(t, [&](int i) { return at[i]; }, top, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
   }
   beam_write<TRACK>(a, tr, g, mol, won_s[wave], fin, place_s[wave], lane);
 }
