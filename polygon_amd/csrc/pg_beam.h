@@ -319,5 +319,6 @@ __device__ __forceinline__ void beam_write(const BeamSelect& a, const BeamTrack&
   if (TRACK) { tr.parent[om] = key ? parent : to; tr.token[om] = v; }
 }
 
-// One step of a search over short vocabularies (V <= 128): logits fp32 [positions, K, ld].
-int launch_beam_track(const BeamSelect& a, const BeamTrack& tr, hipStream_t st);
+// One step of a search (V <= 128): h [positions * K, H] times fcw [64 or 128, H] plus fcb, then the selection.
+template <typename T>
+int launch_beam_head(const BeamSelect& a, const BeamTrack& tr, const T* h, int H, const T* fcw, const float* fcb, hipStream_t st);

@@ -2,6 +2,8 @@
 #include <math.h>
 #include "pg_beam.h"
 #include "pg_host.h"
+#include "pg_mma.h"
+#include <type_traits>
 
 // ---- short vocabularies (V <= 128) ------------------------------------------------------------------------------------
 // 16 lanes hold a row (E = 4 or 8 neighbouring symbols per lane, one wide load), a wave 4 rows at a time, P <= 2 times: a wave
@@ -9,21 +11,22 @@
 // of them), all of softmax's reductions are inside 16 lanes (DPP).  With G > 1 the first wave selects from the G waves' best.
 // Bound by instructions: about half of them the selection, a quarter the 64-bit exponentials.
 constexpr int SW = 4;      // waves per workgroup
+template <int P> struct ShortLds {
+  unsigned long long list[SW][128], won[SW][PG_MAX_BEAMS];
+  double sum[SW][4 * P];
+  int place[SW][PG_MAX_BEAMS], many[SW];
+};
+// Group g (none if !here), whose K rows of logits start at `logits` (global memory or LDS), by the G waves wave, wave + 1, .. of
+// the workgroup (wave % G is one's place among them).  With G > 1 every wave of the workgroup must call it.
 template <typename T, int E, int P, int G, bool TRACK>
-__global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a, BeamTrack tr) {
-  __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
-  __shared__ double sum_s[SW][4 * P];
-  __shared__ int place_s[SW][PG_MAX_BEAMS];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const long g = ((long)blockIdx.x * SW + wave) / G;
-  const int n = TRACK ? min(a.n, *tr.n_dev) : a.n;
-  if (G == 1 && g >= n) return;               // (G > 1: such a wave has no open beam, and takes part in the barrier)
-  const long mol = TRACK && g < n ? tr.mol[g] : g;
+__device__ __forceinline__ void beam_short(const BeamSelect& a, const BeamTrack& tr, const T* logits, long ld, long g, bool here, int wave,
+                                           int lane, ShortLds<P>& lds) {
   const int K = a.K, V = a.V, k0 = wave % G * (4 * P), row = lane >> 4;
+  const long mol = TRACK && here ? tr.mol[g] : g;
   // beam `lane`
   float s_mine = -INFINITY;
   bool fin_mine = false;
-  if (lane < K && (G == 1 || g < n)) {
+  if (here && lane < K) {
     s_mine = a.scores[mol * K + lane];
     fin_mine = a.finished && a.finished[mol * K + lane];
   }
@@ -37,7 +40,7 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
 #pragma unroll
     for (int e = 0; e < E; ++e) x[p][e] = -INFINITY;
     if (!(open >> k & 1) || sub >= V) continue;
-    const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row + v0;
+    const T* r = logits + k * ld + v0;
     const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row + v0 : nullptr;
     if (V >= E) {
       T t[E];
@@ -65,18 +68,18 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
 #pragma unroll
     for (int e = 0; e < E; ++e) sum += beam_exp2(((double)x[p][e] - (double)m[p]) * a.scale);
     sum = sum16(sum);
-    if ((lane & 15) == 0) sum_s[wave][p * 4 + row] = sum;
+    if ((lane & 15) == 0) lds.sum[wave][p * 4 + row] = sum;
   }
   wave_sync();
   // one logarithm for all rows
-  if (lane < 4 * P) sum_s[wave][lane] = beam_log(sum_s[wave][lane]);
+  if (lane < 4 * P) lds.sum[wave][lane] = beam_log(lds.sum[wave][lane]);
   wave_sync();
   float c[P * E], best = -INFINITY;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int k = k0 + p * 4 + row;
     const float s = __shfl(s_mine, k);
-    const double lse = sum_s[wave][p * 4 + row];
+    const double lse = lds.sum[wave][p * 4 + row];
     const bool has = (open >> k & 1) && isfinite(m[p]), done = alive & fin & (1u << k);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -86,27 +89,90 @@ __global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a
       best = fmaxf(best, f);
     }
   }
+  unsigned long long *list = lds.list[wave], *won = lds.won[wave];
   auto index = [&](int i) { return (unsigned)(k0 + i / E * 4 + row) << 20 | (unsigned)(v0 + i % E); };
-  if (G == 1) beam_best<P * E>(c, index, best, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
+  if (G == 1) beam_best<P * E>(c, index, best, -INFINITY, K, list, 0, won, lane);
   else {   // every wave's few, unranked; the group's first wave selects from them
-    __shared__ int many_s[SW];
-    const int many = beam_collect<P * E>(c, index, best, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
-    if (lane == 0) many_s[wave] = many;
+    const int many = beam_collect<P * E>(c, index, best, -INFINITY, K, list, 0, won, lane);
+    if (lane == 0) lds.many[wave] = many;
     __syncthreads();
-    if (wave % G != 0 || g >= n) return;
+    if (wave % G != 0) return;
     float t[2 * G], top = -INFINITY;
     unsigned at[2 * G];
 #pragma unroll
     for (int i = 0; i < 2 * G; ++i) {
       const int j = lane + i % 2 * 64;
-      const unsigned long long key = j < many_s[wave + i / 2] ? list_s[wave + i / 2][j] : 0;
+      const unsigned long long key = j < lds.many[wave + i / 2] ? lds.list[wave + i / 2][j] : 0;
       t[i] = key ? beam_key_number(key) : -INFINITY;
       at[i] = beam_key_index(key);
       top = fmaxf(top, t[i]);
     }
-    beam_best<2 * G>(t, [&](int i) { return at[i]; }, top, -INFINITY, K, list_s[wave], 0, won_s[wave], lane);
+    beam_best<2 * G>(t, [&](int i) { return at[i]; }, top, -INFINITY, K, list, 0, won, lane);
   }
-  beam_write<TRACK>(a, tr, g, mol, won_s[wave], fin, place_s[wave], lane);
+  if (here) beam_write<TRACK>(a, tr, g, mol, won, fin, lds.place[wave], lane);
+}
+template <typename T, int E, int P, int G>
+__global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a) {
+  __shared__ ShortLds<P> lds;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const long g = ((long)blockIdx.x * SW + wave) / G;
+  if (G == 1 && g >= a.n) return;
+  beam_short<T, E, P, G, false>(a, BeamTrack{}, (const T*)a.logits + g * a.ld_group, a.ld_row, g, g < a.n, wave, lane, lds);
+}
+
+// A search's step from the top layer's states: vocabulary projection and selection in one launch.  A workgroup takes the whole
+// groups that fit 32 rows (one tile of the matrix instruction); its four waves contract every fourth 16-byte chunk of H each,
+// straight from memory (the weights, 64 KB in bf16, stay in the L2s), their partial logits meet in LDS, and the selection reads
+// them there.  For few rows it is bound by latency (a projection by the tiled product took 8.6 us and the selection 4.5).
+template <typename T, int E, int P, int G>
+__global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTrack tr, const T* __restrict__ h, int H,
+                                                            const T* __restrict__ fcw, const float* __restrict__ fcb) {
+  constexpr int VP = 16 * E, NT = VP / 32, LD = VP + 4, EPC = 16 / sizeof(T);
+  __shared__ ShortLds<P> lds;
+  __shared__ __attribute__((aligned(16))) float part[2][32][LD];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, K = a.K;
+  const int n = min(a.n, *tr.n_dev), per = 32 / K;
+  const long g0 = (long)blockIdx.x * per;
+  if (g0 >= n) return;                                  // uniform over the workgroup
+  const int rows = (int)min((long)per, n - g0) * K;
+  const int r = lane & 31, half = lane >> 5;
+  const T* hr = h + (g0 * K + min(r, rows - 1)) * H + half * EPC;
+  const T* wr = fcw + (long)r * H + half * EPC;
+  f32x16 acc[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+#pragma unroll 4
+  for (int k = wave * 2 * EPC; k < H; k += SW * 2 * EPC) {      // (H is a multiple of 32)
+    const uint4 x = *reinterpret_cast<const uint4*>(hr + k);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) MmaOp<T>::run(acc[t], x, *reinterpret_cast<const uint4*>(wr + (long)t * 32 * H + k));
+  }
+  // the four partial sums through two tiles (four would not leave room for a second workgroup at 128 symbols)
+  for (int turn = 0; turn < 2; ++turn) {
+    if (wave >> 1 == turn) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float* y = &part[wave & 1][(i & 3) + 8 * (i >> 2) + 4 * half][t * 32 + r];
+          *y = turn ? *y + acc[t][i] : acc[t][i];
+        }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 32 * VP; i += 64 * SW) {
+    const int y = i / VP, v = i % VP;
+    part[0][y][v] = part[0][y][v] + part[1][y][v] + fcb[v];
+  }
+  __syncthreads();
+  for (int q = 0; q < per; q += SW / G) {
+    const int mine = q + wave / G;
+    const bool here = mine < per && g0 + mine < n;
+    beam_short<float, E, P, G, true>(a, tr, &part[0][here ? mine * K : 0][0], LD, g0 + mine, here, wave, lane, lds);
+    if (G > 1) __syncthreads();
+  }
 }
 
 // ---- long vocabularies ------------------------------------------------------------------------------------------------
@@ -435,23 +501,39 @@ extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V)
   return align_up(lists * sizeof(BeamChunk), 256) + lists * K * 8;
 }
 
-template <typename T, bool TRACK> static int launch_short(const BeamSelect& a, const BeamTrack& tr, hipStream_t st) {
-  auto go = [&](auto kernel, int G) { hipLaunchKernelGGL(kernel, dim3(cdiv((long)a.n * G, SW)), dim3(64 * SW), 0, st, a, tr); };
-  const bool narrow = a.V <= 64;
-  if (a.K <= 4) narrow ? go(beam_select_short_kernel<T, 4, 1, 1, TRACK>, 1) : go(beam_select_short_kernel<T, 8, 1, 1, TRACK>, 1);
-  else if (a.K <= 8) narrow ? go(beam_select_short_kernel<T, 4, 2, 1, TRACK>, 1) : go(beam_select_short_kernel<T, 8, 2, 1, TRACK>, 1);
-  else if (a.K <= 16) narrow ? go(beam_select_short_kernel<T, 4, 2, 2, TRACK>, 2) : go(beam_select_short_kernel<T, 8, 2, 2, TRACK>, 2);
-  else narrow ? go(beam_select_short_kernel<T, 4, 2, 4, TRACK>, 4) : go(beam_select_short_kernel<T, 8, 2, 4, TRACK>, 4);
+// f(kernel shape): the narrowest one that holds V symbols and K beams
+template <class F> static void with_short_shape(int V, int K, F f) {
+  auto e = [&](auto p, auto g) {
+    if (V <= 64) f(std::integral_constant<int, 4>{}, p, g);
+    else f(std::integral_constant<int, 8>{}, p, g);
+  };
+  using std::integral_constant;
+  if (K <= 4) e(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  else if (K <= 8) e(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+  else if (K <= 16) e(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+  else e(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+}
+template <typename T> static int launch_short(const BeamSelect& a, hipStream_t st) {
+  with_short_shape(a.V, a.K, [&](auto e, auto p, auto g) {
+    hipLaunchKernelGGL((beam_select_short_kernel<T, e, p, g>), dim3(cdiv((long)a.n * g, SW)), dim3(64 * SW), 0, st, a);
+  });
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
-int launch_beam_track(const BeamSelect& a, const BeamTrack& tr, hipStream_t st) {
-  PG_REQUIRE(a.V <= SHORT_V && a.K <= PG_MAX_BEAMS, "beam search: V=%d or K=%d out of range", a.V, a.K);
-  return launch_short<float, true>(a, tr, st);
+template <typename T>
+int launch_beam_head(const BeamSelect& a, const BeamTrack& tr, const T* h, int H, const T* fcw, const float* fcb, hipStream_t st) {
+  PG_REQUIRE(a.V <= SHORT_V && a.K <= PG_MAX_BEAMS && H % 32 == 0, "beam search: V=%d, K=%d or H=%d out of range", a.V, a.K, H);
+  with_short_shape(a.V, a.K, [&](auto e, auto p, auto g) {
+    hipLaunchKernelGGL((beam_head_kernel<T, e, p, g>), dim3(cdiv(a.n, 32 / a.K)), dim3(64 * SW), 0, st, a, tr, h, H, fcw, fcb);
+  });
+  PG_CHECK_LAUNCH();
+  return PG_OK;
 }
+template int launch_beam_head<float>(const BeamSelect&, const BeamTrack&, const float*, int, const float*, const float*, hipStream_t);
+template int launch_beam_head<bf16_t>(const BeamSelect&, const BeamTrack&, const bf16_t*, int, const bf16_t*, const float*, hipStream_t);
 
 template <typename T> static int beam_select_t(const BeamSelect& a, void* ws, size_t ws_bytes, hipStream_t st) {
-  if (a.V <= SHORT_V) return launch_short<T, false>(a, BeamTrack{}, st);
+  if (a.V <= SHORT_V) return launch_short<T>(a, st);
   const size_t need = pg_beam_select_workspace_bytes(0, a.n, a.K, a.V);
   if (!ws || ws_bytes < need) PG_FAIL(PG_ERR_WORKSPACE, "pg_beam_select: workspace too small (%zu < %zu)", ws_bytes, need);
   BeamLong l = long_plan(a.n, a.K, a.V);

@@ -1,7 +1,7 @@
 // VAE.beam_search: the K most probable strings of every latent, by beam search over the GRU decoder.
 //
-// A row is one beam: group (molecule) p's beams are rows p*K .. p*K + K-1.  Per step: L GRU cells, vocabulary projection,
-// selection (pg_beam.hip, places kept), reorder of the 2 L state planes (only beams with more than one child move).  Beams
+// A row is one beam: group (molecule) p's beams are rows p*K .. p*K + K-1.  Per step: L GRU cells, vocabulary projection
+// and selection (pg_beam.hip, one launch, places kept), reorder of the 2 L state planes (only beams with more than one child move).  Beams
 // end at different lengths: every COMPACT_EVERY steps the molecules whose beams have all ended leave, and the others close
 // up, so the cells run over a shrinking prefix whose length only the device knows - nothing is waited for.  What is recorded
 // per step is a parent and a symbol per beam (2 bytes); the strings are traced back at the end.
@@ -20,7 +20,7 @@ int shadow_join(hipStream_t st);   // pg_vae.hip
 constexpr int COMPACT_EVERY = 8;
 
 struct SearchWs {
-  size_t zop, zproj, h0_32, h0_op, carry[PG_MAX_LAYERS], hop[PG_MAX_LAYERS][2], logits, tok, parents, mol, count, live, last, scores,
+  size_t zop, zproj, h0_32, h0_op, carry[PG_MAX_LAYERS], hop[PG_MAX_LAYERS][2], tok, parents, mol, count, live, last, scores,
       finished, hist, compact, total;
 };
 static SearchWs search_ws_layout(const pg_dims* d, int dtype, long n, int K, int max_len) {
@@ -33,7 +33,6 @@ static SearchWs search_ws_layout(const pg_dims* d, int dtype, long n, int K, int
     w.carry[l] = take(rows * Hd * 4);
     w.hop[l][0] = take(rows * Hd * es); w.hop[l][1] = take(rows * Hd * es);
   }
-  w.logits = take(rows * vpad(d) * 4);
   w.tok = take(rows * 4); w.parents = take(rows * 4);
   w.mol = take(n * 4); w.count = take(2 * 4); w.live = take(n); w.last = take(n * 4);
   w.scores = take(rows * 4); w.finished = take(rows);
@@ -94,7 +93,7 @@ static int search_t(const pg_dims* d, int dtype, const float* params, const void
   const ParamOff po = param_offsets(d);
   const ShadowOff so = shadow_offsets(d, dtype);
   const SearchWs w = search_ws_layout(d, dtype, n, K, max_len);
-  const int Hd = d->Hd, Dz = d->Dz, L = d->L, Vp = vpad(d), rows = n * K;
+  const int Hd = d->Hd, Dz = d->Dz, L = d->L, rows = n * K;
   const long es = sizeof(T);
   int *tok = at<int>(ws, w.tok), *mol = at<int>(ws, w.mol), *count = at<int>(ws, w.count), *last = at<int>(ws, w.last);
   float* beam_scores = at<float>(ws, w.scores);
@@ -151,15 +150,10 @@ static int search_t(const pg_dims* d, int dtype, const float* params, const void
       a.h32 = at<float>(ws, w.carry[l]);
       PG_TRY(launch_gru_fwd<T>(a, st));
     }
-    {
-      GemmEpi<T> e;
-      e.bias = at<float>(shadow, so.fc_b); e.C32 = at<float>(ws, w.logits); e.ldc = Vp;
-      PG_TRY(launch_gemm_nt<T>(at<T>(ws, w.hop[L - 1][p ^ 1]), Hd, at<T>(shadow, so.fc_w), Hd, rows, Vp, Hd, e, st));
-    }
-    const BeamSelect sel = {at<float>(ws, w.logits), (long)K * Vp, Vp, n, K, d->V, allowed, 0, 0, 1.0 / temp, BEAM_LOG2E / temp,
-                            beam_scores, finished, d->eos, d->pad, 1, beam_scores, at<int>(ws, w.parents), tok, finished};
+    const BeamSelect sel = {nullptr, 0, 0, n, K, d->V, allowed, 0, 0, 1.0 / temp, BEAM_LOG2E / temp, beam_scores, finished, d->eos, d->pad,
+                            1, beam_scores, at<int>(ws, w.parents), tok, finished};
     const BeamTrack tr = {count + cur, mol, hist + (long)(i - 1) * rows, hist + half + (long)(i - 1) * rows, live, last, i};
-    PG_TRY(launch_beam_track(sel, tr, st));
+    PG_TRY(launch_beam_head<T>(sel, tr, at<T>(ws, w.hop[L - 1][p ^ 1]), Hd, at<T>(shadow, so.fc_w), at<float>(shadow, so.fc_b), st));
     if (i + 1 == max_len) break;
     pg_plane planes[2 * PG_MAX_LAYERS + 3];
     int np = 0;

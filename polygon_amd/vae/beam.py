@@ -149,7 +149,7 @@ def _planes(planes, what):
 
 
 def _index(t, dev, what):
-    if t.dtype != torch.int32 or t.device != dev:
+    if t.dtype is not torch.int32 or t.device != dev:
         raise ValueError("%s must be int32 on %s, got %s on %s" % (what, dev, t.dtype, t.device))
     return t.contiguous()
 
@@ -170,9 +170,12 @@ def fork_pages(dst, src, index):
     number of times; a negative index or one behind the last page leaves page i as it is).  dst and src share no memory."""
     d, dev, P = _planes(dst, "fork_pages: dst")
     s, sdev, Q = _planes(src, "fork_pages: src")
-    if len(dst) != len(src) or sdev != dev or any(a.dtype != b.dtype or a.shape[1:] != b.shape[1:] for a, b in zip(dst, src)):
+    same = len(dst) == len(src) and sdev == dev
+    for a, b in zip(dst, src):
+        same = same and a.dtype is b.dtype and a.shape[1:] == b.shape[1:]
+    if not same:
         raise ValueError("fork_pages: dst and src must have the same planes but for the number of pages")
-    if tuple(index.shape) != (P,):
+    if index.shape != (P,):
         raise ValueError("index %s does not name a page for each of %d" % (list(index.shape), P))
     index = _index(index, dev, "index")
     _call(dev, _entries().pg_pages_fork, d, s, len(dst), P, Q, index.data_ptr())

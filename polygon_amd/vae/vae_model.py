@@ -789,9 +789,9 @@ class VAE(nn.Module):
         if z.dim() != 2 or z.shape[1] != self.d_z:
             raise RuntimeError("z must be [n, %d], got %s" % (self.d_z, list(z.shape)))
         n, V = z.shape[0], len(self.vocabulary)
-        with torch.no_grad():
+        dev = eng.ensure_flat().device
+        with torch.no_grad(), torch.cuda.device(dev):
             eng.ensure_shadow()
-            dev = eng.flat.device
             z = z.to(dev, torch.float32).contiguous()
             if allowed is not None:
                 if tuple(allowed.shape) != (V,):
