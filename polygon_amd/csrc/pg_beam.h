@@ -127,6 +127,17 @@ __device__ __forceinline__ double sum64(double x) {
   x = sum16(x);
   return (readlane_d(x, 0) + readlane_d(x, 16)) + (readlane_d(x, 32) + readlane_d(x, 48));
 }
+// over the N = 16, 32 or 64 neighbouring lanes that hold a row
+template <int N> __device__ __forceinline__ float max_row(float x) {
+  if (N == 64) return max64(x);
+  x = max16(x);
+  return N == 32 ? fmaxf(x, __shfl_xor(x, 16)) : x;
+}
+template <int N> __device__ __forceinline__ double sum_row(double x) {
+  if (N == 64) return sum64(x);
+  x = sum16(x);
+  return N == 32 ? x + __shfl_xor(x, 16) : x;
+}
 __device__ __forceinline__ unsigned long long max64(unsigned long long x) {
   for (int o = 32; o; o >>= 1) {
     const unsigned long long t = __shfl_xor(x, o);
@@ -176,6 +187,7 @@ __device__ __forceinline__ float beam_bound(float best, float above, int K) {
 // Ranks `m` <= 128 different keys of list[] and puts the K best into won[] in order (won[] beyond m: 0).
 __device__ __forceinline__ void beam_rank(const unsigned long long* list, int m, unsigned long long* won, int K, int lane) {
   if (lane < K) won[lane] = 0;
+  wave_sync();
   const unsigned long long a = lane < m ? list[lane] : 0;
   int ra = 0;
   if (m <= 64) {

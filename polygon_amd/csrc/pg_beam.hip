@@ -5,23 +5,24 @@
 #include "pg_mma.h"
 #include <type_traits>
 
-// ---- short vocabularies (V <= 128) ------------------------------------------------------------------------------------
-// 16 lanes hold a row (E = 4 or 8 neighbouring symbols per lane, one wide load), a wave 4 rows at a time, P <= 2 times: a wave
-// takes up to 8 of a group's rows and a group G = 1, 2 or 4 waves.  The logits are read once and stay in registers (at most 16
-// of them), all of softmax's reductions are inside 16 lanes (DPP).  With G > 1 the first wave selects from the G waves' best.
-// Bound by instructions: about half of them the selection, a quarter the 64-bit exponentials.
-constexpr int SW = 4;      // waves per workgroup
-template <int P> struct ShortLds {
-  unsigned long long list[SW][128], won[SW][PG_MAX_BEAMS];
-  double sum[SW][4 * P];
-  int place[SW][PG_MAX_BEAMS], many[SW];
+// ---- short vocabularies (V <= 1024) -----------------------------------------------------------------------------------
+// N = 16, 32 or 64 lanes hold a row (E neighbouring symbols per lane, wide loads), a wave 64 / N rows at a time, P times, and a
+// group takes the G waves that its K rows need.  The logits are read once and stay in registers (at most 32 of them), and
+// softmax's reductions stay inside a wave (for N = 16 inside DPP rows).  With G > 1 the first wave selects from the G waves'
+// few best.  Bound by instructions: about half of them the selection, a quarter the 64-bit exponentials.
+constexpr int SW = 4;      // waves per workgroup, where G is not more
+template <int W, int ROWS> struct ShortLds {
+  unsigned long long list[W][128], won[W][PG_MAX_BEAMS];
+  double sum[W][ROWS];
+  int place[W][PG_MAX_BEAMS], many[W];
 };
 // Group g (none if !here), whose K rows of logits start at `logits` (global memory or LDS), by the G waves wave, wave + 1, .. of
 // the workgroup (wave % G is one's place among them).  With G > 1 every wave of the workgroup must call it.
-template <typename T, int E, int P, int G, bool TRACK>
+template <typename T, int N, int E, int P, int G, bool TRACK, int W>
 __device__ __forceinline__ void beam_short(const BeamSelect& a, const BeamTrack& tr, const T* logits, long ld, long g, bool here, int wave,
-                                           int lane, ShortLds<P>& lds) {
-  const int K = a.K, V = a.V, k0 = wave % G * (4 * P), row = lane >> 4;
+                                           int lane, ShortLds<W, 64 / N * P>& lds) {
+  constexpr int R = 64 / N;
+  const int K = a.K, V = a.V, k0 = wave % G * (R * P), row = lane / N;
   const long mol = TRACK && here ? tr.mol[g] : g;
   // beam `lane`
   float s_mine = -INFINITY;
@@ -32,11 +33,11 @@ __device__ __forceinline__ void beam_short(const BeamSelect& a, const BeamTrack&
   }
   const unsigned fin = (unsigned)__ballot(fin_mine), alive = (unsigned)__ballot(isfinite(s_mine)), open = alive & ~fin;
   // the lane's symbols v0 .. v0+E-1 of its rows; the row's last lane reads the last E, and leaves out those it shares
-  const int sub = (lane & 15) * E, v0 = min(sub, max(V - E, 0));
+  const int sub = lane % N * E, v0 = min(sub, max(V - E, 0));
   float x[P][E], m[P];
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    const int k = k0 + p * 4 + row;
+    const int k = k0 + p * R + row;
 #pragma unroll
     for (int e = 0; e < E; ++e) x[p][e] = -INFINITY;
     if (!(open >> k & 1) || sub >= V) continue;
@@ -63,23 +64,23 @@ __device__ __forceinline__ void beam_short(const BeamSelect& a, const BeamTrack&
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const float mx = max_nan(x[p]);
-    m[p] = max16(mx != mx ? INFINITY : mx);    // a NaN or +inf makes the row's maximum +inf, and the beam has no continuation
+    m[p] = max_row<N>(mx != mx ? INFINITY : mx);    // a NaN or +inf makes the row's maximum +inf, and the beam has no continuation
     double sum = 0.0;
 #pragma unroll
     for (int e = 0; e < E; ++e) sum += beam_exp2(((double)x[p][e] - (double)m[p]) * a.scale);
-    sum = sum16(sum);
-    if ((lane & 15) == 0) lds.sum[wave][p * 4 + row] = sum;
+    sum = sum_row<N>(sum);
+    if (lane % N == 0) lds.sum[wave][p * R + row] = sum;
   }
   wave_sync();
   // one logarithm for all rows
-  if (lane < 4 * P) lds.sum[wave][lane] = beam_log(lds.sum[wave][lane]);
+  if (lane < R * P) lds.sum[wave][lane] = beam_log(lds.sum[wave][lane]);
   wave_sync();
   float c[P * E], best = -INFINITY;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
-    const int k = k0 + p * 4 + row;
+    const int k = k0 + p * R + row;
     const float s = __shfl(s_mine, k);
-    const double lse = lds.sum[wave][p * 4 + row];
+    const double lse = lds.sum[wave][p * R + row];
     const bool has = (open >> k & 1) && isfinite(m[p]), done = alive & fin & (1u << k);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -90,7 +91,7 @@ __device__ __forceinline__ void beam_short(const BeamSelect& a, const BeamTrack&
     }
   }
   unsigned long long *list = lds.list[wave], *won = lds.won[wave];
-  auto index = [&](int i) { return (unsigned)(k0 + i / E * 4 + row) << 20 | (unsigned)(v0 + i % E); };
+  auto index = [&](int i) { return (unsigned)(k0 + i / E * R + row) << 20 | (unsigned)(v0 + i % E); };
   if (G == 1) beam_best<P * E>(c, index, best, -INFINITY, K, list, 0, won, lane);
   else {   // every wave's few, unranked; the group's first wave selects from them
     const int many = beam_collect<P * E>(c, index, best, -INFINITY, K, list, 0, won, lane);
@@ -111,13 +112,14 @@ __device__ __forceinline__ void beam_short(const BeamSelect& a, const BeamTrack&
   }
   if (here) beam_write<TRACK>(a, tr, g, mol, won, fin, lds.place[wave], lane);
 }
-template <typename T, int E, int P, int G>
-__global__ __launch_bounds__(64 * SW) void beam_select_short_kernel(BeamSelect a) {
-  __shared__ ShortLds<P> lds;
+template <typename T, int N, int E, int P, int G>
+__global__ __launch_bounds__(64 * (G > SW ? G : SW)) void beam_select_short_kernel(BeamSelect a) {
+  constexpr int W = G > SW ? G : SW;
+  __shared__ ShortLds<W, 64 / N * P> lds;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const long g = ((long)blockIdx.x * SW + wave) / G;
+  const long g = ((long)blockIdx.x * W + wave) / G;
   if (G == 1 && g >= a.n) return;
-  beam_short<T, E, P, G, false>(a, BeamTrack{}, (const T*)a.logits + g * a.ld_group, a.ld_row, g, g < a.n, wave, lane, lds);
+  beam_short<T, N, E, P, G, false>(a, BeamTrack{}, (const T*)a.logits + g * a.ld_group, a.ld_row, g, g < a.n, wave, lane, lds);
 }
 
 // A search's step from the top layer's states: vocabulary projection and selection in one launch.  A workgroup takes the whole
@@ -128,7 +130,7 @@ template <typename T, int E, int P, int G>
 __global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTrack tr, const T* __restrict__ h, int H,
                                                             const T* __restrict__ fcw, const float* __restrict__ fcb) {
   constexpr int VP = 16 * E, NT = VP / 32, LD = VP + 4, EPC = 16 / sizeof(T);
-  __shared__ ShortLds<P> lds;
+  __shared__ ShortLds<SW, 4 * P> lds;
   __shared__ __attribute__((aligned(16))) float part[2][32][LD];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, K = a.K;
   const int n = min(a.n, *tr.n_dev), per = 32 / K;
@@ -170,34 +172,35 @@ __global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTr
   for (int q = 0; q < per; q += SW / G) {
     const int mine = q + wave / G;
     const bool here = mine < per && g0 + mine < n;
-    beam_short<float, E, P, G, true>(a, tr, &part[0][here ? mine * K : 0][0], LD, g0 + mine, here, wave, lane, lds);
+    beam_short<float, 16, E, P, G, true>(a, tr, &part[0][here ? mine * K : 0][0], LD, g0 + mine, here, wave, lane, lds);
     if (G > 1) __syncthreads();
   }
 }
 
 // ---- long vocabularies ------------------------------------------------------------------------------------------------
-// The vocabulary is split into chunks; a wave walks through its chunk in tiles of 64 x 8 or 16 symbols held in registers, with a
-// running maximum and 64-bit sum of the softmax and the K best logits so far (a tile's symbols at or below the K-th best are
-// out at one comparison per lane).  A chunk leaves (max, sum, K keys of logit and symbol).  A workgroup per group then joins
-// the chunks' sums, turns their keys into scores and selects.
+// The vocabulary is split into chunks; a wave walks through its chunk in tiles of 64 x 16 symbols held in registers, with a
+// running maximum and 64-bit sum of the softmax and the K + 1 best logits so far (a tile's symbols at or below the last of them
+// are out at one comparison per lane).  A chunk leaves (max, sum, K + 1 keys of logit and symbol).  A workgroup per group then
+// joins the chunks' sums, turns their keys into scores and selects.  Where that would be many keys for one workgroup (few
+// groups, many chunks), a workgroup per row first merges the row's chunks into one.
+constexpr int LE = 16, TILE = 64 * LE, LONG_KEYS = PG_MAX_BEAMS + 1;
 struct BeamChunk {
   double sum;
   float max;       // +inf: a NaN or +inf was seen
   int pad;
 };
 struct BeamLong {
-  int tile, tiles, chunks;       // symbols of a tile; tiles of a chunk; chunks of a row
+  int tiles, chunks;             // tiles of a chunk; chunks of a row
   BeamChunk* part;               // [n * K, chunks]
-  unsigned long long* keys;      // [n * K, chunks, K]
+  unsigned long long* keys;      // [n * K, chunks, K + 1], best first, 0 behind the last
 };
-template <typename T, int LE>
+template <typename T>
 __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamLong l) {
-  constexpr int TILE = 64 * LE;
-  __shared__ unsigned long long list_s[SW][128], won_s[SW][PG_MAX_BEAMS];
+  __shared__ unsigned long long list_s[SW][128], won_s[SW][LONG_KEYS];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const long u = (long)blockIdx.x * SW + __builtin_amdgcn_readfirstlane(wave);
   const long row = u / l.chunks;
-  const int chunk = (int)(u - row * l.chunks), K = a.K, V = a.V;
+  const int chunk = (int)(u - row * l.chunks), K = a.K, V = a.V, L = K + 1;
   if (row >= (long)a.n * K) return;
   if (!isfinite(a.scores[row]) || (a.finished && a.finished[row])) return;     // the join does not look at this row
   const long g = row / K;
@@ -208,15 +211,16 @@ __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamL
   float mx = -INFINITY;
   double sum = 0.0;
   bool bad = false;
-  float above = -INFINITY;       // the K-th best so far (-inf: fewer than K)
+  float above = -INFINITY;       // the last of the L best so far (-inf: fewer than L)
   unsigned long long *list = list_s[wave], *won = won_s[wave];
-  int m = 0;                     // keys in list[], at most 48 between tiles: the K best when it was last ranked, and later ones
+  bool fresh = false;            // there are keys behind the ranked ones
+  int m = 0;                     // keys in list[], at most 48 between tiles: the L best when it was last ranked, and later ones
   auto settle = [&]() {          // won[] becomes the list
-    const unsigned long long key = lane < K ? won[lane] : 0;
+    const unsigned long long key = lane < L ? won[lane] : 0;
     if (key) list[lane] = key;
     m = __popcll(__ballot(key != 0));
-    const unsigned kth = __builtin_amdgcn_readlane((int)(key >> 32), K - 1);
-    above = kth ? beam_unorder(kth) : -INFINITY;
+    const unsigned last = __builtin_amdgcn_readlane((int)(key >> 32), L - 1);
+    above = last ? beam_unorder(last) : -INFINITY;
     wave_sync();
   };
   for (int t = 0; t < l.tiles; ++t) {
@@ -259,7 +263,7 @@ __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamL
       if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // four at a time: enough to hide their latency, and few registers
     }
     if (!__ballot(top > above)) continue;
-    // what the tile has above the K-th best is put behind the K best, and the list is ranked when it has grown: a stale bound
+    // what the tile has above the last of the best is put behind them, and the list is ranked when it has grown: a stale bound
     // lets a few more in, which is cheaper than a ranking per tile
     const int m0 = m;
     if (__popcll(__ballot(top > above)) <= 32) {
@@ -273,23 +277,87 @@ __global__ __launch_bounds__(64 * SW) void beam_chunk_kernel(BeamSelect a, BeamL
           m += __popcll(some);
         }
       }
+      fresh = m > m0 || fresh;
       if (m <= 48) continue;
     }
-    if (m > m0 && m <= 128) beam_rank(list, m, won, K, lane);
-    else beam_best<LE>(x, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, top, above, K, list, m0, won, lane);
+    if (m > m0 && m <= 128) beam_rank(list, m, won, L, lane);
+    else beam_best<LE>(x, [&](int i) { return (unsigned)(b + (i / W * 64 + lane) * W + i % W); }, top, above, L, list, m0, won, lane);
     settle();
+    fresh = false;
   }
-  if (m > K) { beam_rank(list, m, won, K, lane); settle(); }
+  if (fresh) { beam_rank(list, m, won, L, lane); settle(); }
   const bool any_bad = __ballot(bad) != 0;
   sum = sum64(sum);
   if (lane == 0) l.part[row * l.chunks + chunk] = {sum, any_bad ? INFINITY : mx, 0};
-  if (lane < K) l.keys[(row * l.chunks + chunk) * K + lane] = lane < m ? list[lane] : 0;
+  if (lane < L) l.keys[(row * l.chunks + chunk) * L + lane] = lane < m ? list[lane] : 0;
+}
+
+// One workgroup per row: its chunks' maxima, sums and keys become those of one chunk, l2's.
+__global__ __launch_bounds__(64 * SW) void beam_merge_kernel(BeamSelect a, BeamLong l, BeamLong l2) {
+  constexpr int B = 8;           // keys per lane and turn
+  __shared__ unsigned long long list_s[SW][128], won_s[SW][LONG_KEYS];
+  __shared__ int many[SW];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, L = a.K + 1;
+  const long row = blockIdx.x;
+  if (!isfinite(a.scores[row]) || (a.finished && a.finished[row])) return;
+  if (wave == 0) {
+    const BeamChunk* part = l.part + row * l.chunks;
+    float mx = -INFINITY;
+    double sum = 0.0;
+    for (int c = lane; c < l.chunks; c += 64) mx = fmaxf(mx, part[c].max);
+    mx = max64(mx);
+    if (isfinite(mx))
+      for (int c = lane; c < l.chunks; c += 64) sum += part[c].sum * beam_exp2(((double)part[c].max - (double)mx) * a.scale);
+    sum = sum64(sum);
+    if (lane == 0) l2.part[row] = {sum, mx, 0};
+  }
+  // every wave the best of its turns (the chunks, and so the symbols, ascend: an equal logit that comes later has the higher
+  // index and stays out), then the four lists
+  const unsigned long long* keys = l.keys + row * (long)l.chunks * L;
+  unsigned long long *list = list_s[wave], *won = won_s[wave];
+  const int total = l.chunks * L;
+  float above = -INFINITY;
+  int m = 0;
+  for (int e0 = wave * 64 * B; e0 < total; e0 += SW * 64 * B) {
+    float x[B], top = -INFINITY;
+    unsigned at[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int e = e0 + i * 64 + lane;
+      const unsigned long long key = e < total ? keys[e] : 0;
+      x[i] = key ? beam_key_number(key) : -INFINITY;
+      at[i] = beam_key_index(key);
+      top = fmaxf(top, x[i]);
+    }
+    if (!__ballot(top > above)) continue;
+    beam_best<B>(x, [&](int i) { return at[i]; }, top, above, L, list, m, won, lane);
+    const unsigned long long key = lane < L ? won[lane] : 0;
+    if (key) list[lane] = key;
+    m = __popcll(__ballot(key != 0));
+    const unsigned last = __builtin_amdgcn_readlane((int)(key >> 32), L - 1);
+    above = last ? beam_unorder(last) : -INFINITY;
+    wave_sync();
+  }
+  if (lane == 0) many[wave] = m;
+  __syncthreads();
+  if (wave != 0) return;
+  // (4 x 33 keys would not fit the 128 that a ranking takes: two by two)
+  for (int w = 1; w < SW; ++w) {
+    if (lane < many[w]) list[m + lane] = list_s[w][lane];
+    wave_sync();
+    beam_rank(list, m + many[w], won, L, lane);
+    const unsigned long long key = lane < L ? won[lane] : 0;
+    if (key) list[lane] = key;
+    m = __popcll(__ballot(key != 0));
+    wave_sync();
+  }
+  if (lane < L) l2.keys[row * L + lane] = lane < m ? list[lane] : 0;
 }
 
 // One workgroup per group.  The first JKEEP entries of every thread are loaded before anything else and stay in registers (that
-// is all of them unless K * K * chunks > 2048), their latency behind the rows' sums, which 16 lanes each work out.
+// is all of them: more are merged first), their latency behind the rows' sums, which 16 lanes each work out.
 // Bound by latency: a chain of loads, two exchanges through LDS, and the ranking of some 2 K keys.
-constexpr int JW = 4, JLIST = 1024, JKEEP = 8;
+constexpr int JW = 4, JLIST = 1024, JKEEP = 10;
 template <typename T>
 __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLong l) {
   __shared__ unsigned long long list[JLIST], won[PG_MAX_BEAMS], red[JW];
@@ -299,7 +367,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   __shared__ unsigned best_s[64 * JW];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, K = a.K, V = a.V;
   const long g = blockIdx.x;
-  const int per_row = l.chunks * K, total = K * per_row;
+  const int L = K + 1, per_row = l.chunks * L, total = K * per_row;
   const unsigned long long* keys = l.keys + g * (long)total;
   float s_mine = -INFINITY;
   bool fin_mine = false;
@@ -333,14 +401,13 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   }
   if (tid == 0) have = 0;
   __syncthreads();
-  // entry e of the group's K * chunks * K, as a key of its score (0: none)
+  // entry e of the group's K * chunks * L, as a key of its score (0: none)
   auto scored = [&](int e, unsigned long long key) -> unsigned long long {
     const int k = e / per_row;
     if (!key || !isfinite(max_s[k])) return 0;
     const float c = beam_score(beam_key_number(key), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
     return c > -INFINITY ? beam_key(c, (unsigned)k << 20 | beam_key_index(key)) : 0;
   };
-  auto entry = [&](int e) -> unsigned long long { return open >> (e / per_row) & 1 ? scored(e, keys[e]) : 0; };
   auto ended = [&](int k) -> unsigned long long {      // a finished beam's own candidate
     return alive & fin & (1u << k) ? beam_key(score_s[k], (unsigned)k << 20 | (unsigned)a.pad) : 0;
   };
@@ -351,7 +418,6 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     if (tid < K) f(ended(tid));
 #pragma unroll
     for (int i = 0; i < JKEEP; ++i) f(kept[i]);
-    for (int e = tid + JKEEP * 64 * JW; e < total; e += 64 * JW) f(entry(e));
   };
   // a bound that at least K of the threads' bests reach (found in every wave alike)
   unsigned best = 0;
@@ -421,9 +487,9 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   }
   __syncthreads();
   // A chunk's list goes by the logit, the selection by the score, and rounding can give symbols with different logits one
-  // score: then the lower index counts.  What a full list left out can only matter if the list's last entry has exactly the
-  // score of the group's last winner (a better one would make K + 1 winners); such a chunk is read again for the symbols of
-  // that score.  It takes all of a group's winners coming from one chunk.
+  // score: then the lower index counts.  What a list left out can only matter if its last entry, the K + 1st, still has the score of
+  // the group's last winner (it cannot have a better one: K others of the list are as good) and a lower logit could have it too;
+  // such a chunk is read again for the symbols of that score.  (Logits that tie by being equal are listed by index already.)
   const unsigned edge = (unsigned)(won[K - 1] >> 32);
   if (edge == 0) {
     if (wave == 0) beam_write<false>(a, BeamTrack{}, g, g, won, fin, place, lane);
@@ -433,9 +499,19 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
     if (tid == 0) have = 0;
     __syncthreads();
     {
-      const int kc = base + tid;       // (beam, chunk); one that starts behind the last winner cannot hold a lower index
-      if (kc < K * l.chunks && (unsigned)(entry(kc * K + K - 1) >> 32) == edge &&
-          ((unsigned)(kc / l.chunks) << 20 | (unsigned)(kc % l.chunks) * l.tiles * l.tile) < beam_key_index(won[K - 1]))
+      const int kc = base + tid, k = kc / l.chunks;       // (beam, chunk)
+      bool near = false;
+      if (kc < K * l.chunks && (open >> k & 1)) {
+        const unsigned long long key = keys[kc * L + K];
+        // the list's last entry has the edge's score, so has the next lower number of the logits' type, and the chunk does not
+        // start behind the last winner
+        if ((unsigned)(scored(kc * L + K, key) >> 32) == edge) {
+          const float lower = beam_unorder((unsigned)(key >> 32) - (sizeof(T) == 2 ? 0x10000u : 1u));
+          near = (unsigned)(beam_key(beam_score(lower, max_s[k], a.inv_temp, lse_s[k], score_s[k]), 0) >> 32) == edge &&
+                 ((unsigned)k << 20 | (unsigned)(kc % l.chunks) * l.tiles * TILE) < beam_key_index(won[K - 1]);
+        }
+      }
+      if (near)
         again[atomicAdd(&have, 1)] = kc;
     }
     __syncthreads();
@@ -444,12 +520,12 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
       const int k = again[i] / l.chunks, c = again[i] % l.chunks;
       const T* r = (const T*)a.logits + g * a.ld_group + k * a.ld_row;
       const uint8_t* mk = a.mask ? a.mask + g * a.mask_group + k * a.mask_row : nullptr;
-      const long v1 = min((long)V, (long)(c + 1) * l.tiles * l.tile);
+      const long v1 = min((long)V, (long)(c + 1) * l.tiles * TILE);
       // the symbols of the edge's score, lowest first, until one does not beat the last winner
       unsigned long long last = ~0ull;
       for (int round = 0; round < K; ++round) {
         unsigned long long top = 0;
-        for (long v = (long)c * l.tiles * l.tile + tid; v < v1; v += 64 * JW) {
+        for (long v = (long)c * l.tiles * TILE + tid; v < v1; v += 64 * JW) {
           if (mk && !mk[v]) continue;
           const float sc = beam_score(to_f32<T>(r[v]), max_s[k], a.inv_temp, lse_s[k], score_s[k]);
           const unsigned long long key = beam_key(sc, (unsigned)k << 20 | (unsigned)v);
@@ -481,50 +557,69 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   if (wave == 0) beam_write<false>(a, BeamTrack{}, g, g, won, fin, place, lane);
 }
 
-constexpr int SHORT_V = 128;
+constexpr int SHORT_V = 1024;
 // Tiles per chunk: as long as there are waves enough for the card (8 on each of its 1024 SIMDs) a chunk is made longer - the
 // K best so far make the next tile cheap, and there are fewer lists to join.
 static BeamLong long_plan(int n, int K, int V) {
   BeamLong l = {};
-  l.tile = V <= 512 ? 512 : 1024;
-  const long tiles = (V + l.tile - 1) / l.tile, rows = (long)n * K;
+  const long tiles = (V + TILE - 1) / TILE, rows = (long)n * K;
   l.tiles = (int)std::max<long>(1, std::min<long>(tiles, rows * tiles / 4096));
   l.chunks = (int)((tiles + l.tiles - 1) / l.tiles);
   return l;
 }
 
-extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V) {
-  (void)dtype;
-  if (n < 1 || K < 1 || V <= SHORT_V) return 0;
-  const BeamLong l = long_plan(n, K, V);
-  const size_t lists = (size_t)n * K * l.chunks;
-  return align_up(lists * sizeof(BeamChunk), 256) + lists * K * 8;
+// A group's keys that its one workgroup of the join takes without a merge: what it holds in registers.  Measured, a whole call: one
+// group, K = 16, 131072 symbols (34816 keys) 27 us with the merge and 117 without; four groups, K = 8, 32001 symbols (2304) 20.7
+// with and 18.0 without.
+static bool long_merges(const BeamLong& l, int K) { return l.chunks > 1 && (long)K * (K + 1) * l.chunks > JKEEP * 64 * JW; }
+struct LongWs { size_t part, keys, part2, keys2, total; };
+static LongWs long_ws(const BeamLong& l, int n, int K) {
+  LongWs w;
+  size_t p = 0;
+  auto take = [&](size_t bytes) { size_t r = p; p = align_up(p + bytes, 256); return r; };
+  const size_t rows = (size_t)n * K, merged = long_merges(l, K) ? rows : 0;
+  w.part = take(rows * l.chunks * sizeof(BeamChunk)); w.keys = take(rows * l.chunks * (K + 1) * 8);
+  w.part2 = take(merged * sizeof(BeamChunk)); w.keys2 = take(merged * (K + 1) * 8);
+  w.total = p;
+  return w;
 }
 
-// f(kernel shape): the narrowest one that holds V symbols and K beams
+extern "C" size_t pg_beam_select_workspace_bytes(int dtype, int n, int K, int V) {
+  (void)dtype;
+  return n < 1 || K < 1 || V <= SHORT_V ? 0 : long_ws(long_plan(n, K, V), n, K).total;
+}
+
+template <int I> using Int = std::integral_constant<int, I>;
+// Waves per group: the least power of two whose waves of `rows` rows each hold K
+template <class F> static void with_waves(int K, int rows, F f) {
+  if (K <= rows) f(Int<1>{});
+  else if (K <= 2 * rows) f(Int<2>{});
+  else if (K <= 4 * rows) f(Int<4>{});
+  else if (K <= 8 * rows) f(Int<8>{});
+  else f(Int<16>{});
+}
+// f(N, E, P, G): the narrowest kernel that holds V symbols and K beams
 template <class F> static void with_short_shape(int V, int K, F f) {
-  auto e = [&](auto p, auto g) {
-    if (V <= 64) f(std::integral_constant<int, 4>{}, p, g);
-    else f(std::integral_constant<int, 8>{}, p, g);
-  };
-  using std::integral_constant;
-  if (K <= 4) e(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-  else if (K <= 8) e(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-  else if (K <= 16) e(integral_constant<int, 2>{}, integral_constant<int, 2>{});
-  else e(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+  auto shape = [&](auto n, auto e, auto p) { with_waves(K, 64 / n * p, [&](auto g) { if constexpr (g * (64 / n * p) <= PG_MAX_BEAMS) f(n, e, p, g); }); };
+  if (V <= 64) K <= 4 ? f(Int<16>{}, Int<4>{}, Int<1>{}, Int<1>{}) : shape(Int<16>{}, Int<4>{}, Int<2>{});
+  else if (V <= 128) K <= 4 ? f(Int<16>{}, Int<8>{}, Int<1>{}, Int<1>{}) : shape(Int<16>{}, Int<8>{}, Int<2>{});
+  else if (V <= 256) shape(Int<32>{}, Int<8>{}, Int<4>{});
+  else if (V <= 512) shape(Int<64>{}, Int<8>{}, Int<4>{});
+  else shape(Int<64>{}, Int<16>{}, Int<2>{});
 }
 template <typename T> static int launch_short(const BeamSelect& a, hipStream_t st) {
-  with_short_shape(a.V, a.K, [&](auto e, auto p, auto g) {
-    hipLaunchKernelGGL((beam_select_short_kernel<T, e, p, g>), dim3(cdiv((long)a.n * g, SW)), dim3(64 * SW), 0, st, a);
+  with_short_shape(a.V, a.K, [&](auto n, auto e, auto p, auto g) {
+    constexpr int W = g > SW ? g : SW;
+    hipLaunchKernelGGL((beam_select_short_kernel<T, n, e, p, g>), dim3(cdiv((long)a.n * g, W)), dim3(64 * W), 0, st, a);
   });
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
 template <typename T>
 int launch_beam_head(const BeamSelect& a, const BeamTrack& tr, const T* h, int H, const T* fcw, const float* fcb, hipStream_t st) {
-  PG_REQUIRE(a.V <= SHORT_V && a.K <= PG_MAX_BEAMS && H % 32 == 0, "beam search: V=%d, K=%d or H=%d out of range", a.V, a.K, H);
-  with_short_shape(a.V, a.K, [&](auto e, auto p, auto g) {
-    hipLaunchKernelGGL((beam_head_kernel<T, e, p, g>), dim3(cdiv(a.n, 32 / a.K)), dim3(64 * SW), 0, st, a, tr, h, H, fcw, fcb);
+  PG_REQUIRE(a.V <= PG_MAX_V && a.K <= PG_MAX_BEAMS && H % 32 == 0, "beam search: V=%d, K=%d or H=%d out of range", a.V, a.K, H);
+  with_short_shape(a.V, a.K, [&](auto n, auto e, auto p, auto g) {
+    if constexpr (n == 16) hipLaunchKernelGGL((beam_head_kernel<T, e, p, g>), dim3(cdiv(a.n, 32 / a.K)), dim3(64 * SW), 0, st, a, tr, h, H, fcw, fcb);
   });
   PG_CHECK_LAUNCH();
   return PG_OK;
@@ -534,17 +629,24 @@ template int launch_beam_head<bf16_t>(const BeamSelect&, const BeamTrack&, const
 
 template <typename T> static int beam_select_t(const BeamSelect& a, void* ws, size_t ws_bytes, hipStream_t st) {
   if (a.V <= SHORT_V) return launch_short<T>(a, st);
-  const size_t need = pg_beam_select_workspace_bytes(0, a.n, a.K, a.V);
-  if (!ws || ws_bytes < need) PG_FAIL(PG_ERR_WORKSPACE, "pg_beam_select: workspace too small (%zu < %zu)", ws_bytes, need);
   BeamLong l = long_plan(a.n, a.K, a.V);
-  const long lists = (long)a.n * a.K * l.chunks;
+  const LongWs w = long_ws(l, a.n, a.K);
+  if (!ws || ws_bytes < w.total) PG_FAIL(PG_ERR_WORKSPACE, "pg_beam_select: workspace too small (%zu < %zu)", ws_bytes, w.total);
+  const long rows = (long)a.n * a.K, lists = rows * l.chunks;
   PG_REQUIRE(lists < (1L << 26), "pg_beam_select: n=%d, K=%d, V=%d are too many rows for one call", a.n, a.K, a.V);
-  l.part = at<BeamChunk>(ws, 0);
-  l.keys = at<unsigned long long>(ws, align_up((size_t)lists * sizeof(BeamChunk), 256));
-  const dim3 grid(cdiv(lists, SW)), block(64 * SW);
-  if (l.tile == 512) hipLaunchKernelGGL((beam_chunk_kernel<T, 8>), grid, block, 0, st, a, l);
-  else hipLaunchKernelGGL((beam_chunk_kernel<T, 16>), grid, block, 0, st, a, l);
+  l.part = at<BeamChunk>(ws, w.part);
+  l.keys = at<unsigned long long>(ws, w.keys);
+  hipLaunchKernelGGL(beam_chunk_kernel<T>, dim3(cdiv(lists, SW)), dim3(64 * SW), 0, st, a, l);
   PG_CHECK_LAUNCH();
+  if (long_merges(l, a.K)) {
+    BeamLong l2 = l;
+    l2.tiles = l.tiles * l.chunks; l2.chunks = 1;
+    l2.part = at<BeamChunk>(ws, w.part2);
+    l2.keys = at<unsigned long long>(ws, w.keys2);
+    hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)rows), dim3(64 * SW), 0, st, a, l, l2);
+    PG_CHECK_LAUNCH();
+    l = l2;
+  }
   hipLaunchKernelGGL(beam_join_kernel<T>, dim3(a.n), dim3(64 * JW), 0, st, a, l);
   PG_CHECK_LAUNCH();
   return PG_OK;

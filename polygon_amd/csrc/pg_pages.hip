@@ -2,12 +2,15 @@
 #include "pg_pages.h"
 #include "pg_host.h"
 
-// What a move kernel needs of a cache: its planes, and where each plane's first column segment is counted.  A segment is
-// PG_SEG bytes of a page: 16 bytes for each lane of a wave.
+// What a move kernel needs of a cache: its planes, and how their columns are dealt out to waves.  A lane takes 16 bytes, so a wave
+// covers PG_SEG = 1024 bytes of one page, or - pages of at most 512 bytes - 64 / lanes neighbouring groups of pages at once
+// (lanes: the power of two that holds one).  Units are counted in blocks of 64 groups: a block has 64 * segments units of a wide
+// plane and `lanes` of a narrow one; first[] is where each plane's begin.
 constexpr int PG_SEG = 1024;
 struct Planes {
   pg_plane p[PG_MAX_PLANES];
   int first[PG_MAX_PLANES + 1];
+  int lanes[PG_MAX_PLANES];        // 64: a wide plane
   int n;
 };
 static int make_planes(const char* who, const pg_plane* planes, int n, Planes* out) {
@@ -15,12 +18,26 @@ static int make_planes(const char* who, const pg_plane* planes, int n, Planes* o
   for (int i = 0; i < n; ++i) {
     out->p[i] = planes[i];
     out->first[i] = (int)at;
-    at += (planes[i].bytes + PG_SEG - 1) / PG_SEG;
-    PG_REQUIRE(at < (1L << 30), "%s: pages of more than 2^40 bytes", who);
+    int lanes = 1;
+    while (lanes < 64 && lanes * 16L < planes[i].bytes) lanes *= 2;
+    out->lanes[i] = lanes;
+    at += lanes == 64 ? 64 * ((planes[i].bytes + PG_SEG - 1) / PG_SEG) : lanes;
+    PG_REQUIRE(at < (1L << 30), "%s: pages of more than 2^34 bytes", who);
   }
   out->first[n] = (int)at;
   out->n = n;
   return PG_OK;
+}
+static bool any_narrow(const Planes& pl) {
+  for (int i = 0; i < pl.n; ++i)
+    if (pl.lanes[i] < 64) return true;
+  return false;
+}
+// MIX: some planes are narrow, and units are dealt out in blocks of 64 groups.  Otherwise group by group, with less arithmetic and
+// fewer registers per wave (measured with 9 KB pages, all wide: 77 us so, 95 us in blocks; with pages of 64 and 128 bytes a wave
+// per group and plane took 146 us, blocks 65).
+template <bool MIX> __host__ __device__ __forceinline__ long plane_units(const Planes& pl, long groups) {
+  return MIX ? (groups + 63) / 64 * pl.first[pl.n] : groups * (pl.first[pl.n] / 64);
 }
 
 // Two planes of `pages` pages share bytes: their spans overlap, unless they interleave with one pitch.
@@ -63,44 +80,81 @@ __device__ __forceinline__ void page_store(unsigned char* p, long left, const ui
   if (left & 2) { const unsigned short h = (unsigned short)v.w; __builtin_memcpy(p + o, &h, 2); o += 2; }
   if (left & 1) p[o] = (unsigned char)(v.w >> 16);
 }
-// plane and column of segment `seg` (wave-uniform)
-__device__ __forceinline__ int seg_plane(const Planes& pl, int seg) {
-  int i = 0;
-  while (i + 1 < pl.n && seg >= pl.first[i + 1]) ++i;
-  return i;
+// A lane's place in unit u: plane i (wave-uniform), group g, column col.  wide: g is the wave's (uniform).
+struct Place {
+  int i;
+  bool wide;
+  long g, col;
+};
+template <bool MIX> __device__ __forceinline__ Place unit_place(const Planes& pl, long u, int lane) {
+  const int per = MIX ? pl.first[pl.n] : pl.first[pl.n] / 64;
+  const long block = u / per;
+  int r = (int)(u - block * per);
+  if (!MIX) r *= 64;
+  Place p;
+  p.i = 0;
+  while (p.i + 1 < pl.n && r >= pl.first[p.i + 1]) ++p.i;
+  r -= pl.first[p.i];
+  p.wide = !MIX || pl.lanes[p.i] == 64;
+  if (!MIX) {
+    p.g = block;
+    p.col = (long)(r / 64) * PG_SEG + lane * 16;
+  } else if (p.wide) {
+    const int segs = (pl.first[p.i + 1] - pl.first[p.i]) / 64, q = r / segs;
+    p.g = block * 64 + q;
+    p.col = (long)(r - q * segs) * PG_SEG + lane * 16;
+  } else {
+    p.g = block * 64 + (r * 64 + lane) / pl.lanes[p.i];
+    p.col = lane % pl.lanes[p.i] * 16;
+  }
+  return p;
 }
 
-// Moves of pages: R pages at a time in one column segment, one wave; every load of a wave is issued before its first store.
+// Moves of pages: R pages at a time in one column segment; every load of a wave is issued before its first store.
 // REORDER: the R pages are a group's K (<= R) and the sources lie among them, so whatever the parents are no page is
 // overwritten before all of the segment's sources are in registers, and no other wave touches this segment of the group.
 // Pages that keep their state are not touched.  Fork: the R pages are consecutive pages of dst, their sources pages of src.
-// Bound by HBM: 16 bytes per lane, up to R loads in flight per wave.
-template <int R, bool REORDER>
-__global__ __launch_bounds__(256) void pages_move_kernel(Planes dst, Planes src, long units, int K, long n_dst, unsigned n_src,
+// Bound by HBM where pages are wide: 16 bytes per lane, up to R loads in flight per wave.
+template <int R, bool REORDER, bool MIX>
+__global__ __launch_bounds__(256) void pages_move_kernel(Planes dst, Planes src, long groups, int K, long n_dst, unsigned n_src,
                                                          const int32_t* __restrict__ from, const int* __restrict__ groups_dev) {
   const int lane = threadIdx.x & 63;
-  const int segs = dst.first[dst.n];
-  if (groups_dev) units = min(units, (long)*groups_dev * segs);
+  if (groups_dev) groups = min(groups, (long)*groups_dev);
+  const long units = plane_units<MIX>(dst, groups);
   for (long u = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); u < units; u += (long)gridDim.x * 4) {
-    const long g = u / segs;
-    const int seg = (int)(u - g * segs), i = seg_plane(dst, seg);
-    const long col = (long)(seg - dst.first[i]) * PG_SEG + lane * 16, left = dst.p[i].bytes - col;
-    const long page0 = g * K, dp = dst.p[i].pitch, sp = REORDER ? dp : src.p[i].pitch;
-    unsigned char* d = (unsigned char*)dst.p[i].base + page0 * dp + col;
-    const unsigned char* s = REORDER ? d : (const unsigned char*)src.p[i].base + col;
-    const int mine = lane < K && page0 + lane < n_dst ? from[page0 + lane] : -1;
+    const Place at = unit_place<MIX>(dst, u, lane);
+    const long left = at.g < groups ? dst.p[at.i].bytes - at.col : 0;
+    const long page0 = at.g * K, dp = dst.p[at.i].pitch, sp = REORDER ? dp : src.p[at.i].pitch;
+    unsigned char* d = (unsigned char*)dst.p[at.i].base + page0 * dp + at.col;
+    const unsigned char* s = REORDER ? d : (const unsigned char*)src.p[at.i].base + at.col;
     int f[R];
     uint4 v[R];
+    if (at.wide) {          // one group: its sources are scalars
+      const int mine = lane < K && at.g < groups && page0 + lane < n_dst ? from[page0 + lane] : -1;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-      f[j] = __builtin_amdgcn_readlane(mine, j);
-      const bool moves = j < K && (unsigned)f[j] < (REORDER ? (unsigned)K : n_src) && !(REORDER && f[j] == j);
-      f[j] = moves ? f[j] : -1;
-      if (f[j] >= 0 && left > 0) v[j] = page_load(s + f[j] * sp, left);
+      for (int j = 0; j < R; ++j) f[j] = __builtin_amdgcn_readlane(mine, j);
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const bool moves = j < K && (unsigned)f[j] < (REORDER ? (unsigned)K : n_src) && !(REORDER && f[j] == j);
+        f[j] = moves ? f[j] : -1;
+        if (f[j] >= 0 && left > 0) v[j] = page_load(s + f[j] * sp, left);
+      }
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        if (f[j] >= 0 && left > 0) page_store(d + j * dp, left, v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < R; ++j) f[j] = j < K && left > 0 && page0 + j < n_dst ? from[page0 + j] : -1;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const bool moves = j < K && (unsigned)f[j] < (REORDER ? (unsigned)K : n_src) && !(REORDER && f[j] == j);
+        f[j] = moves ? f[j] : -1;
+        if (f[j] >= 0) v[j] = page_load(s + f[j] * sp, left);
+      }
+#pragma unroll
+      for (int j = 0; j < R; ++j)
+        if (f[j] >= 0) page_store(d + j * dp, left, v[j]);
     }
-#pragma unroll
-    for (int j = 0; j < R; ++j)
-      if (f[j] >= 0 && left > 0) page_store(d + j * dp, left, v[j]);
   }
 }
 // waves of 4 per workgroup; more units than this many workgroups hold are taken in rounds
@@ -145,29 +199,27 @@ template <int NT> __device__ __forceinline__ int block_before(int x, int* total,
   *total = t;
   return b + s - x;
 }
-// The moves, one wave per MV consecutive column segments: MV loads in flight, then the stores.
+// The moves ("groups" of one page), one wave per MV consecutive units: MV loads in flight, then the stores.
 constexpr int MV = 4;
-template <typename I>
+template <bool MIX, typename I>
 __device__ __forceinline__ void move_pages(const Planes& pl, long moves, const I* hole, const I* mover) {
-  const int lane = threadIdx.x & 63, segs = pl.first[pl.n];
-  const long items = moves * segs;
-  for (long u = ((long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * MV; u < items; u += (long)gridDim.x * 4 * MV) {
+  const int lane = threadIdx.x & 63;
+  const long units = plane_units<MIX>(pl, moves);
+  for (long u = ((long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * MV; u < units; u += (long)gridDim.x * 4 * MV) {
     uint4 v[MV];
     unsigned char* to[MV];
     long left[MV];
-    long m = u / segs;
-    int seg = (int)(u - m * segs);
 #pragma unroll
     for (int j = 0; j < MV; ++j) {
       left[j] = 0;
-      if (u + j < items) {
-        const int i = seg_plane(pl, seg);
-        const long col = (long)(seg - pl.first[i]) * PG_SEG + lane * 16;
-        left[j] = pl.p[i].bytes - col;
-        const unsigned char* from = (const unsigned char*)pl.p[i].base + mover[m] * pl.p[i].pitch + col;
-        to[j] = (unsigned char*)pl.p[i].base + hole[m] * pl.p[i].pitch + col;
-        if (left[j] > 0) v[j] = page_load(from, left[j]);
-        if (++seg == segs) { seg = 0; ++m; }
+      if (u + j < units) {
+        const Place at = unit_place<MIX>(pl, u + j, lane);
+        if (at.g < moves) {
+          const pg_plane& p = pl.p[at.i];
+          left[j] = p.bytes - at.col;
+          to[j] = (unsigned char*)p.base + hole[at.g] * p.pitch + at.col;
+          if (left[j] > 0) v[j] = page_load((const unsigned char*)p.base + mover[at.g] * p.pitch + at.col, left[j]);
+        }
       }
     }
 #pragma unroll
@@ -175,11 +227,15 @@ __device__ __forceinline__ void move_pages(const Planes& pl, long moves, const I
       if (left[j] > 0) page_store(to[j], left[j], v[j]);
   }
 }
-static int compact_grid(long n, long segs) { return (int)std::max<long>(1, std::min<long>((n / 2 * segs + 4 * MV - 1) / (4 * MV), 2048)); }
+static int compact_grid(const Planes& pl, bool mix, long n) {
+  const long units = mix ? plane_units<true>(pl, n / 2) : plane_units<false>(pl, n / 2);
+  return (int)std::max<long>(1, std::min<long>((units + 4 * MV - 1) / (4 * MV), 2048));
+}
 
 // Up to PLAN_PAGES pages: ONE launch, every workgroup works the plan out for itself (n flag bytes from L2, a scan, the moves'
 // ends as 16-bit lists in LDS) and takes its share of the moves.
 constexpr int PLAN_PAGES = 16384;
+template <bool MIX>
 __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, const int* __restrict__ n_dev,
                                                             const uint8_t* __restrict__ live, int32_t* __restrict__ count,
                                                             int32_t* __restrict__ map) {
@@ -220,7 +276,7 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, co
     const bool l = bits[t] >> i & 1;
     map[p] = !l ? -1 : p < total ? p : (int)hole[before[t] + __popcll(bits[t] & ((1ull << i) - 1)) - low];
   }
-  move_pages(pl, moves, hole, mover);
+  move_pages<MIX>(pl, moves, hole, mover);
 }
 
 // More pages: the plan by one workgroup into the workspace, then the moves.
@@ -257,23 +313,26 @@ __global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const int* __re
   if (map)
     for (int i = tid; i < total - low; i += 1024) map[mover[i]] = hole[i];
 }
+template <bool MIX>
 __global__ __launch_bounds__(256) void pages_compact_move_kernel(Planes pl, const int32_t* __restrict__ moves,
                                                                  const int32_t* __restrict__ hole, const int32_t* __restrict__ mover) {
-  move_pages(pl, moves[0], hole, mover);
+  move_pages<MIX>(pl, moves[0], hole, mover);
 }
 
 int launch_pages_reorder(const pg_plane* planes, int n_planes, int n_groups, const int* groups_dev, int K, const int32_t* parents,
                          hipStream_t st) {
   Planes pl;
   PG_TRY(make_planes("pg_pages_reorder", planes, n_planes, &pl));
-  const long units = (long)n_groups * pl.first[n_planes], pages = (long)n_groups * K;
+  const long pages = (long)n_groups * K;
   // R registers of 16 bytes per lane: the narrowest instantiation that holds the group
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(move_grid(units)), dim3(256), 0, st, pl, pl, units, K, pages, 0u, parents, groups_dev);
+  const bool mix = any_narrow(pl);
+  const int grid = move_grid(mix ? plane_units<true>(pl, n_groups) : plane_units<false>(pl, n_groups));
+  auto go = [&](auto mixed, auto plain) {
+    hipLaunchKernelGGL(mix ? mixed : plain, dim3(grid), dim3(256), 0, st, pl, pl, (long)n_groups, K, pages, 0u, parents, groups_dev);
   };
-  if (K <= 8) go(pages_move_kernel<8, true>);
-  else if (K <= 16) go(pages_move_kernel<16, true>);
-  else go(pages_move_kernel<32, true>);
+  if (K <= 8) go(pages_move_kernel<8, true, true>, pages_move_kernel<8, true, false>);
+  else if (K <= 16) go(pages_move_kernel<16, true, true>, pages_move_kernel<16, true, false>);
+  else go(pages_move_kernel<32, true, true>, pages_move_kernel<32, true, false>);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
@@ -304,9 +363,11 @@ extern "C" int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_pla
   PG_TRY(make_planes("pg_pages_fork", dst, n_planes, &d));
   PG_TRY(make_planes("pg_pages_fork", src, n_planes, &s));
   constexpr int R = 8;
-  const long units = (long)cdiv(n_dst, R) * d.first[n_planes];
-  hipLaunchKernelGGL((pages_move_kernel<R, false>), dim3(move_grid(units)), dim3(256), 0, (hipStream_t)stream, d, s, units, R, (long)n_dst,
-                     (unsigned)n_src, index, (const int*)nullptr);
+  const long groups = cdiv(n_dst, R);
+  const bool mix = any_narrow(d);
+  const int grid = move_grid(mix ? plane_units<true>(d, groups) : plane_units<false>(d, groups));
+  auto* kernel = mix ? pages_move_kernel<R, false, true> : pages_move_kernel<R, false, false>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, (hipStream_t)stream, d, s, groups, R, (long)n_dst, (unsigned)n_src, index, (const int*)nullptr);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }
@@ -321,16 +382,19 @@ int launch_pages_compact(const pg_plane* planes, int n_planes, int n_pages, cons
                          int32_t* map, void* ws, hipStream_t st) {
   Planes pl;
   PG_TRY(make_planes("pg_pages_compact", planes, n_planes, &pl));
-  const int grid = compact_grid(n_pages, pl.first[n_planes]);
+  const bool mix = any_narrow(pl);
+  const int grid = compact_grid(pl, mix, n_pages);
   if (n_pages <= PLAN_PAGES) {
-    hipLaunchKernelGGL(pages_compact_kernel, dim3(grid), dim3(256), (size_t)(n_pages / 2) * 4, st, pl, n_pages, n_dev, live, count, map);
+    auto* kernel = mix ? pages_compact_kernel<true> : pages_compact_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), (size_t)(n_pages / 2) * 4, st, pl, n_pages, n_dev, live, count, map);
     PG_CHECK_LAUNCH();
     return PG_OK;
   }
   int32_t *moves = at<int32_t>(ws, 0), *hole = at<int32_t>(ws, 256), *mover = at<int32_t>(ws, 256 + compact_list_bytes(n_pages));
   hipLaunchKernelGGL(pages_plan_kernel, dim3(1), dim3(1024), 0, st, n_pages, n_dev, live, count, map, moves, hole, mover);
   PG_CHECK_LAUNCH();
-  hipLaunchKernelGGL(pages_compact_move_kernel, dim3(grid), dim3(256), 0, st, pl, moves, hole, mover);
+  auto* kernel = mix ? pages_compact_move_kernel<true> : pages_compact_move_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, pl, moves, hole, mover);
   PG_CHECK_LAUNCH();
   return PG_OK;
 }

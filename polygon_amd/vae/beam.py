@@ -15,7 +15,7 @@ import torch
 from polygon_amd import _lib
 
 MAX_BEAMS = 32      # PG_MAX_BEAMS
-NO_WORKSPACE_V = 128      # up to here pg_beam_select_workspace_bytes is 0: not asked
+NO_WORKSPACE_V = 1024     # up to here pg_beam_select_workspace_bytes is 0: not asked
 
 
 class BeamStep(NamedTuple):

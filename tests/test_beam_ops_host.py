@@ -106,8 +106,8 @@ def test_wrappers_refuse():
 def test_workspace():
     need = beam._entries().pg_beam_select_workspace_bytes
     assert all(need(t, n, K, beam.NO_WORKSPACE_V) == 0 for t in (0, 1) for n in (1, 10 ** 5) for K in (1, 32))
-    assert need(0, 1, 1, beam.NO_WORKSPACE_V + 1) > 0 and need(0, 0, 4, 1000) == 0
-    assert _select(V=1000, ws=FAKE, ws_bytes=need(0, 1, 2, 1000) - 1) == -4 and _select(V=1000, ws=None, ws_bytes=1 << 20) == -4
+    assert need(0, 1, 1, beam.NO_WORKSPACE_V + 1) > 0 and need(0, 0, 4, 9000) == 0
+    assert _select(V=9000, ws=FAKE, ws_bytes=need(0, 1, 2, 9000) - 1) == -4 and _select(V=9000, ws=None, ws_bytes=1 << 20) == -4
     assert _select(n=1 << 20, K=16) == -1                # n * K not below 2^24
 
 

@@ -74,7 +74,7 @@ def make(n, K, V, dtype=torch.float32, seed=0, dead=0.1, done=0.2):
 
 SHAPES = [(1, 1, 1), (3, 2, 1), (5, 1, 7), (2, 32, 2), (4, 5, 3), (1, 5, 51), (130, 8, 51), (9, 8, 64), (9, 8, 65), (33, 32, 128),
           (17, 31, 127), (3, 7, 129), (5, 16, 257), (2, 32, 512), (3, 4, 1000), (2, 8, 1025), (2, 16, 5003), (1, 3, 40001),
-          (3, 32, 9000)]
+          (3, 32, 9000), (1, 16, 70000)]
 
 
 @pytest.mark.parametrize("keep", [False, True])
@@ -163,6 +163,17 @@ def test_select_ties_made_by_rounding(V):
     mask = torch.ones(V, device="cuda", dtype=torch.bool)
     mask[:5] = False
     check_select(logits, scores, mask=mask)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,K,V", [(9, 5, 51), (5, 8, 250), (4, 16, 900), (3, 8, 3000), (2, 7, 20000), (1, 16, 70000)])
+def test_select_ties_between_and_within_beams(n, K, V, dt):
+    """Scores so large that a step of their rounding spans many logits: most of what is compared is equal"""
+    logits, scores, fin = make(n, K, V, dt, seed=7)
+    for base in (-3.0e4, -1.0e6):
+        s = torch.where(torch.isfinite(scores), scores.mul(0.05).round() + base, scores)
+        check_select(logits, s, finished=fin, eos=1, keep_slots=True)
+        check_select(logits, s[:, :1].expand(n, K))
 
 
 def test_select_strides():
