@@ -9,7 +9,9 @@
 // N = 16, 32 or 64 lanes hold a row (E neighbouring symbols per lane, wide loads), a wave 64 / N rows at a time, P times, and a
 // group takes the G waves that its K rows need.  The logits are read once and stay in registers (at most 32 of them), and
 // softmax's reductions stay inside a wave (for N = 16 inside DPP rows).  With G > 1 the first wave selects from the G waves'
-// few best.  Bound by instructions: about half of them the selection, a quarter the 64-bit exponentials.
+// few best.  Bound by instructions (some 700 a wave at 8 x 51, half of them the selection, a fifth the 64-bit exponentials):
+// 8192 x 8 x 51 fp32 14.4 us for 10.5 MB, 1024 x 32 x 128 bf16 with masks 18.8 us, one group 4.6 us, most of it latency.
+// Measured against the chunked kernels below where those could start: 4096 x 8 x 129 19 us here, 63 there; 2000 x 8 x 1000 28 and 56.
 constexpr int SW = 4;      // waves per workgroup, where G is not more
 template <int W, int ROWS> struct ShortLds {
   unsigned long long list[W][128], won[W][PG_MAX_BEAMS];
@@ -123,9 +125,10 @@ __global__ __launch_bounds__(64 * (G > SW ? G : SW)) void beam_select_short_kern
 }
 
 // A search's step from the top layer's states: vocabulary projection and selection in one launch.  A workgroup takes the whole
-// groups that fit 32 rows (one tile of the matrix instruction); its four waves contract every fourth 16-byte chunk of H each,
+// groups that fit 32 rows (one tile of the matrix instruction); its four waves contract every fourth step of H each,
 // straight from memory (the weights, 64 KB in bf16, stay in the L2s), their partial logits meet in LDS, and the selection reads
-// them there.  For few rows it is bound by latency (a projection by the tiled product took 8.6 us and the selection 4.5).
+// them there.  For few rows it is bound by latency: 9.4 us for one group where the tiled product and the selection took 8.7 and
+// 4.5; 11 instead of 15.4 + 7.2 us at 512 rows, 49 instead of 25 + 13 at 65536 (where the cells take 1500).
 template <typename T, int E, int P, int G>
 __global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTrack tr, const T* __restrict__ h, int H,
                                                             const T* __restrict__ fcw, const float* __restrict__ fcb) {
@@ -183,6 +186,10 @@ __global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTr
 // are out at one comparison per lane).  A chunk leaves (max, sum, K + 1 keys of logit and symbol).  A workgroup per group then
 // joins the chunks' sums, turns their keys into scores and selects.  Where that would be many keys for one workgroup (few
 // groups, many chunks), a workgroup per row first merges the row's chunks into one.
+// 64 x 8 x 131072 fp32 (268 MB): 73.7 us, 3.6 TB/s, and 7.0 us for the join.  Reading alone takes 44 us; the exponentials add 26
+// (17 instructions a symbol; matrix units do not help an exponential), the later tiles' selection 13: the vector units are busy
+// 70 % of the time.  No gain: tiles of 32 symbols a lane (87 us: fewer waves), the next tile loaded ahead into registers (77)
+// or through LDS (70.5), more or fewer waves.
 constexpr int LE = 16, TILE = 64 * LE, LONG_KEYS = PG_MAX_BEAMS + 1;
 struct BeamChunk {
   double sum;

@@ -226,6 +226,69 @@ def test_many_molecules_leave_and_close_up():
     assert (last <= 8).float().mean() > 0.1 and (last == 40).float().mean() > 0.1          # they did leave at different times
 
 
+def test_operators_driven_from_outside():
+    """a program's own decode loop (torch's GRU arithmetic, fp32) over beam_select, reorder_pages, compact_pages and fork_pages
+    finds what VAE.beam_search finds"""
+    from polygon_amd import vae
+    model, P = sharp_model(TINY, 18, "fp32")
+    n, K, T, H, L = 40, 6, 25, TINY["Hd"], TINY["L"]
+    z = torch.randn(n, TINY["Dz"], generator=torch.Generator().manual_seed(9)).cuda()
+    want = [t.cpu() for t in model.beam_search_tokens(z, K, T)]
+    w = {k: torch.from_numpy(v).float().cuda() for k, v in P.items()}
+    start = z @ w["decoder_lat.weight"].T + w["decoder_lat.bias"]
+    planes = [torch.zeros(n * K, H, device="cuda") for _ in range(L)] + [torch.zeros(n * K, T, dtype=torch.uint8, device="cuda")]
+    rows = torch.arange(n, dtype=torch.int32, device="cuda").repeat_interleave(K)
+    vae.fork_pages(planes[:L], [start] * L, rows)
+    zr = z.repeat_interleave(K, 0)
+    tok = torch.full((n, K), model.bos, dtype=torch.int32, device="cuda")
+    planes[L][:, 0] = model.bos
+    scores = torch.full((n, K), -float("inf"), device="cuda")
+    scores[:, 0] = 0
+    fin = torch.zeros(n, K, dtype=torch.bool, device="cuda")
+    mol = torch.arange(n, device="cuda")
+    found = {}
+    for t in range(1, T):
+        x = torch.cat([w["x_emb.weight"][tok.flatten().long()], zr], 1)
+        for l in range(L):
+            gi = x @ w["decoder_rnn.weight_ih_l%d" % l].T + w["decoder_rnn.bias_ih_l%d" % l]
+            gh = planes[l] @ w["decoder_rnn.weight_hh_l%d" % l].T + w["decoder_rnn.bias_hh_l%d" % l]
+            r, u = torch.sigmoid(gi[:, :2 * H] + gh[:, :2 * H]).chunk(2, 1)
+            new = torch.tanh(gi[:, 2 * H:] + r * gh[:, 2 * H:])
+            planes[l].copy_((1 - u) * new + u * planes[l])
+            x = planes[l]
+        y = x @ w["decoder_fc.weight"].T + w["decoder_fc.bias"]
+        step = vae.beam_select(y.view(len(mol), K, -1), scores, fin, eos=model.eos, pad=model.pad, keep_slots=True)
+        vae.reorder_pages(planes, step.parents)
+        scores, fin, tok = step.scores, step.finished, step.tokens
+        planes[L][:, t] = tok.flatten().to(torch.uint8)
+        done = fin.all(1) if t + 1 < T else torch.ones_like(fin[:, 0])
+        if not done.any():
+            continue
+        for i in done.nonzero().flatten().tolist():
+            found[int(mol[i])] = (planes[L].view(len(mol), K, T)[i].cpu(), scores[i].cpu(), t)
+        group = [p.view(len(mol), -1) for p in planes + [zr]]
+        extra = [scores, fin, tok, mol.view(-1, 1)]
+        count, place = vae.compact_pages(group + extra, ~done)
+        m = int(count)
+        if m == 0:
+            break
+        assert m == int((~done).sum()) and torch.equal(place[~done].sort().values.cpu(), torch.arange(m, dtype=torch.int32))
+        planes, zr = [g[:m].reshape(m * K, -1) for g in group[:-1]], group[-1][:m].reshape(m * K, -1)
+        scores, fin, tok, mol = extra[0][:m], extra[1][:m], extra[2][:m], extra[3][:m, 0]
+    assert len(found) == n
+    out = [torch.full((n, K, T), model.pad, dtype=torch.uint8), torch.zeros(n, K, dtype=torch.int32), torch.zeros(n, K)]
+    same = 0
+    for i in range(n):
+        tokens, sc, t = found[i]
+        order = sc.argsort(descending=True, stable=True)
+        out[0][i, :, :t + 1], out[2][i] = tokens[order][:, :t + 1], sc[order]
+        for j, row in enumerate(out[0][i].tolist()):
+            out[1][i, j] = row.index(model.eos) + 1 if model.eos in row else T
+        same += torch.equal(out[0][i], want[0][i])
+    check_scores(P, z.cpu().numpy(), out, "fp32")
+    assert same >= 0.9 * n       # (the rest: beams that two fp32 evaluations order differently)
+
+
 def test_stream_and_graph():
     model, P = sharp_model(TINY, 15, "bf16")
     zs = torch.randn(50, TINY["Dz"], generator=torch.Generator().manual_seed(7)).cuda()
