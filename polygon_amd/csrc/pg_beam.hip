@@ -518,8 +518,7 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
                  ((unsigned)k << 20 | (unsigned)(kc % l.chunks) * l.tiles * TILE) < beam_key_index(won[K - 1]);
         }
       }
-      if (near)
-        again[atomicAdd(&have, 1)] = kc;
+      if (near) again[atomicAdd(&have, 1)] = kc;
     }
     __syncthreads();
     const int again_n = have;
@@ -565,8 +564,8 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
 }
 
 constexpr int SHORT_V = 1024;
-// Tiles per chunk: as long as there are waves enough for the card (8 on each of its 1024 SIMDs) a chunk is made longer - the
-// K best so far make the next tile cheap, and there are fewer lists to join.
+// Tiles per chunk: as long as there are waves enough for the card (4 on each of its 1024 SIMDs) a chunk is made longer - the
+// K + 1 best so far make the next tile cheap, and there are fewer lists to join.
 static BeamLong long_plan(int n, int K, int V) {
   BeamLong l = {};
   const long tiles = (V + TILE - 1) / TILE, rows = (long)n * K;
