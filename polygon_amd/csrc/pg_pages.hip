@@ -61,6 +61,15 @@ static int check_planes(const char* who, const pg_plane* planes, int n_planes, l
   return PG_OK;
 }
 
+// What a call reads as flags or indices, or writes beside the pages, lies outside them: workgroups move pages while others still
+// read the indices.
+static int check_apart(const char* who, const pg_plane* planes, int n_planes, long pages, const char* what, const void* at, long bytes) {
+  for (int i = 0; i < n_planes; ++i)
+    PG_REQUIRE(!planes_share(planes[i], pages, pg_plane{(void*)at, planes[i].pitch, bytes}, bytes > 0), "%s: %s shares bytes with plane %d",
+               who, what, i);
+  return PG_OK;
+}
+
 // One lane's 16 bytes of a page, `left` >= 1 of them inside it.  Any alignment: the hardware takes unaligned wide accesses.
 __device__ __forceinline__ uint4 page_load(const unsigned char* p, long left) {
   uint4 v = {0, 0, 0, 0};
@@ -344,6 +353,7 @@ extern "C" int pg_pages_reorder(const pg_plane* planes, int n_planes, int n_grou
   PG_TRY(check_planes("pg_pages_reorder", planes, n_planes, (long)n_groups * K));
   if (n_groups == 0) return PG_OK;
   PG_REQUIRE(parents, "pg_pages_reorder: parents is NULL");
+  PG_TRY(check_apart("pg_pages_reorder", planes, n_planes, (long)n_groups * K, "parents", parents, (long)n_groups * K * 4));
   return launch_pages_reorder(planes, n_planes, n_groups, nullptr, K, parents, (hipStream_t)stream);
 }
 
@@ -361,6 +371,7 @@ extern "C" int pg_pages_fork(const pg_plane* dst, const pg_plane* src, int n_pla
   }
   if (n_dst == 0 || n_src == 0) return PG_OK;
   PG_REQUIRE(index, "pg_pages_fork: index is NULL");
+  PG_TRY(check_apart("pg_pages_fork", dst, n_planes, n_dst, "index", index, n_dst * 4L));
   Planes d, s;
   PG_TRY(make_planes("pg_pages_fork", dst, n_planes, &d));
   PG_TRY(make_planes("pg_pages_fork", src, n_planes, &s));
@@ -407,5 +418,13 @@ extern "C" int pg_pages_compact(const pg_plane* planes, int n_planes, int n_page
   PG_REQUIRE(count && (n_pages == 0 || (live && map)), "pg_pages_compact: NULL buffer");
   const size_t need = pg_pages_compact_workspace_bytes(n_pages);
   if (ws_bytes < need || (need && !ws)) PG_FAIL(PG_ERR_WORKSPACE, "pg_pages_compact: workspace too small (%zu < %zu)", ws_bytes, need);
+  const struct { const char* what; const void* at; size_t bytes; } beside[] = {
+      {"live", live, (size_t)n_pages}, {"count", count, 4}, {"map", map, n_pages * 4ul}, {"the workspace", ws, need}};
+  for (const auto& b : beside) {
+    PG_TRY(check_apart("pg_pages_compact", planes, n_planes, n_pages, b.what, b.at, (long)b.bytes));
+    for (const auto* o = beside; o < &b; ++o)
+      PG_REQUIRE((uintptr_t)o->at + o->bytes <= (uintptr_t)b.at || (uintptr_t)b.at + b.bytes <= (uintptr_t)o->at || !o->bytes || !b.bytes,
+                 "pg_pages_compact: %s and %s share bytes", o->what, b.what);
+  }
   return launch_pages_compact(planes, n_planes, n_pages, nullptr, live, count, map, ws, (hipStream_t)stream);
 }

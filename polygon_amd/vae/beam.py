@@ -156,7 +156,7 @@ def _index(t, dev, what):
 
 def reorder_pages(planes, parents):
     """In place: page g*K + j of every plane takes over what page g*K + parents[g, j] held before the call.  ``planes``:
-    tensors [n*K, ...], dense behind the first dimension; ``parents`` [n, K] int32 (``BeamStep.parents``)."""
+    tensors [n*K, ...], dense behind the first dimension; ``parents`` [n, K] int32 (``BeamStep.parents``), outside the planes."""
     d, dev, P = _planes(planes, "reorder_pages")
     shape = parents.shape
     if len(shape) != 2 or shape[0] * shape[1] != P:
@@ -167,7 +167,8 @@ def reorder_pages(planes, parents):
 
 def fork_pages(dst, src, index):
     """Page i of ``dst`` becomes a copy of page index[i] of ``src`` in every plane (index int32 [n_dst]; a page may be taken any
-    number of times; a negative index or one behind the last page leaves page i as it is).  dst and src share no memory."""
+    number of times; a negative index or one behind the last page leaves page i as it is).  dst shares no memory with src or
+    index."""
     d, dev, P = _planes(dst, "fork_pages: dst")
     s, sdev, Q = _planes(src, "fork_pages: src")
     same = len(dst) == len(src) and sdev == dev
@@ -184,7 +185,8 @@ def fork_pages(dst, src, index):
 def compact_pages(planes, live):
     """Frees the pages whose ``live`` flag ([P] bool) is not set and closes the gaps, in place: the live pages behind the new
     end move, in order, to the dead places before it.  Returns (count int32 [1], map int32 [P]: the new place of every old
-    page, -1 for a freed one), both on the device."""
+    page, -1 for a freed one), both on the device.  ``live`` is read while pages move: where the flags are a plane themselves,
+    pass a copy."""
     d, dev, P = _planes(planes, "compact_pages")
     live = _flags(live, (P,), dev, "live")
     L = _entries()

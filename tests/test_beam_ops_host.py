@@ -69,6 +69,20 @@ def test_pages_refuse():
     assert need > 0 and compact(ws=None) == compact(size=need - 1) == -4
 
 
+def test_indices_are_no_pages():
+    """flags, parents and indices that lie inside pages that the call moves would change under the workgroups that read them"""
+    L = beam._entries()
+    planes, other = _pl((FAKE + (1 << 16), 128, 64), ONE), _pl((FAKE + (1 << 17), 128, 64), (FAKE + (1 << 18), 64, 64))
+    refused = lambda status: status == -1 and b"share" in L.pg_last_error()  # noqa: E731
+    for at in (FAKE, FAKE + 255, FAKE - 3, FAKE + (1 << 16) + 130, FAKE + (1 << 16) + 60, FAKE + (1 << 16) + 125):
+        assert refused(L.pg_pages_reorder(planes, 2, 2, 2, at, None))
+        assert refused(L.pg_pages_fork(planes, other, 2, 4, 4, at, None))
+        away = FAKE + (1 << 20)
+        for args in ((at, away, away + 64), (away, at, away + 64), (away, away + 64, at), (away, away + 3, away + 64), (away, away + 64, away - 15)):
+            assert refused(L.pg_pages_compact(planes, 2, 4, *args, None, 0, None))
+    assert refused(L.pg_pages_compact(_pl((FAKE, 64, 64)), 1, 1 << 15, FAKE << 4, FAKE << 5, FAKE << 6, FAKE + 640, 1 << 30, None))
+
+
 def test_interleaved_planes_are_told_from_shared_ones():
     """planes of one buffer: columns [0, 64) and [64, 128) of rows of 128 bytes share nothing, whichever comes first"""
     L = beam._entries()

@@ -323,6 +323,38 @@ def test_interleaved_planes():
     assert torch.equal(both[:, 0], both[:, 1])
 
 
+def test_indices_between_and_inside_pages():
+    """flags and parents that share a buffer with the pages: taken where they lie beside them, refused where they are moved too"""
+    full = torch.randint(0, 200, (12, 128), device="cuda", dtype=torch.uint8)
+    old = full.cpu().clone()
+    live, par = full[2, 64:76], full[5, 68:116].view(torch.int32).view(3, 4)
+    flags = torch.tensor([1, 0, 0, 1, 1, 0, 1, 0, 1, 1, 0, 1], dtype=torch.uint8)
+    live.copy_(flags)
+    old[2, 64:76] = flags
+    c, w = ref_compact(flags != 0)
+    count, where = vae.compact_pages([full[:, :64]], live)
+    for p, q in enumerate(w):
+        if q >= 0:
+            old[q, :64] = old[p, :64]
+    assert count.item() == c and where.tolist() == w.tolist() and torch.equal(full[:c, :64].cpu(), old[:c, :64])
+    par.copy_(torch.tensor([[1, 1, 2, 0], [0, 1, 2, 3], [3, 2, 1, 0]], dtype=torch.int32))
+    old, rows = full.cpu().clone(), (par.cpu() + torch.arange(3)[:, None] * 4).flatten()
+    vae.reorder_pages([full[:, :64]], par)
+    assert torch.equal(full[:, :64].cpu(), old[rows][:, :64]) and torch.equal(full[:, 64:].cpu(), old[:, 64:])
+
+    state, alive = torch.randn(6, 40, device="cuda"), torch.ones(6, dtype=torch.bool, device="cuda")
+    parents, other = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(6, dtype=torch.int32, device="cuda")
+    index = torch.zeros(6, dtype=torch.int32, device="cuda")
+    with pytest.raises(PolygonHipError):
+        vae.compact_pages([state, alive], alive)
+    with pytest.raises(PolygonHipError):
+        vae.reorder_pages([state, parents.view(6)], parents)
+    with pytest.raises(PolygonHipError):
+        vae.fork_pages([index], [other], index)
+    vae.compact_pages([state, alive], alive.clone())
+    vae.fork_pages([other], [index], index)               # only read: may be a page
+
+
 def test_far_offsets():
     """pages beyond 2^31 and 2^32 bytes"""
     P = 70000
