@@ -218,8 +218,9 @@ PG_API int pg_beam_select(int dtype, const void* logits, long ld_group, long ld_
  * under softmax(y / temp), and one that reached its eos competes with its score unchanged.  allowed (nullable): V bytes, 0 = the
  * symbol is never taken.  tokens uint8 [n, K, max_len] best first (bos, symbols, eos, pad), end_pads int32 [n, K] as pg_sample's
  * (max_len without an eos; 0 where there are fewer than K hypotheses), scores float [n, K] (-inf there).  max_len >= 2,
- * K <= PG_MAX_BEAMS, n * K < 2^24; about 14 KB of workspace a beam (bf16 default decoder, 8 beams).  Molecules whose beams have all ended
- * leave the decode.  Per-step kernels only: no persistent launch. */
+ * K <= PG_MAX_BEAMS, n * K < 2^24; about 14 KB of workspace a beam (bf16 default decoder, 8 beams).  Latents whose states
+ * (n * K * Hd values of dtype) exceed 2 GiB, or of more than 65535 * 64 beams, are decoded in turns in the workspace of one, so
+ * the workspace stops growing there.  Molecules whose beams have all ended leave the decode.  Per-step kernels only: no persistent launch. */
 PG_API size_t pg_beam_search_workspace_bytes(const pg_dims* d, int dtype, int n, int K, int max_len);
 PG_API int pg_beam_search(const pg_dims* d, int dtype, const float* params, const void* shadow, void* ws, size_t ws_bytes, int n,
                           int K, int max_len, const float* z, const uint8_t* allowed, double temp, uint8_t* tokens,

@@ -20,6 +20,15 @@ int shadow_join(hipStream_t st);   // pg_vae.hip
 // 1024 x 8 12.3 ms, 8192 x 8 77.6 ms (72 of them the cells, 2.8 projection and selection, 2.2 reorder, 0.1 compaction).
 constexpr int COMPACT_EVERY = 8;
 
+// Latents of one turn.  The cells and the products read states and latents by 32-bit byte offsets into a descriptor of 2 GiB, and
+// the cells' grid counts tiles of 64 rows in its second dimension: a call beyond that decodes its latents in turns of one size, one after
+// another in the same workspace.
+static long latent_bytes(const pg_dims* d, int dtype, int K) { return std::max((long)K * d->Hd, (long)d->Dz) * (dtype == PG_BF16 ? 2 : 4); }
+static int turn_size(const pg_dims* d, int dtype, int n, int K) {
+  const long most = std::min(((1L << 31) - 1) / latent_bytes(d, dtype, K), 65535L * 64 / K);
+  return cdiv(n, cdiv(n, most));
+}
+
 struct SearchWs {
   size_t zop, zproj, h0_32, h0_op, carry[PG_MAX_LAYERS], hop[PG_MAX_LAYERS][2], tok, parents, mol, count, live, last, scores,
       finished, hist, compact, total;
@@ -183,10 +192,11 @@ static int check_search(const pg_dims* d, int dtype, int n, int K, int max_len) 
   PG_REQUIRE(n >= 1 && K >= 1 && K <= PG_MAX_BEAMS && (long)n * K < 1L << 24, "pg_beam_search: n=%d, K=%d (K <= %d, n * K < 2^24)", n, K,
              PG_MAX_BEAMS);
   PG_REQUIRE(max_len >= 2 && max_len <= 1 << 20, "pg_beam_search: max_len=%d outside [2, 2^20]", max_len);
+  PG_REQUIRE(latent_bytes(d, dtype, K) < 1L << 31, "pg_beam_search: one latent's %d beams of %d units do not fit an operand of 2 GiB", K, d->Hd);
   return PG_OK;
 }
 extern "C" size_t pg_beam_search_workspace_bytes(const pg_dims* d, int dtype, int n, int K, int max_len) {
-  return check_search(d, dtype, n, K, max_len) == PG_OK ? search_ws_layout(d, dtype, n, K, max_len).total : 0;
+  return check_search(d, dtype, n, K, max_len) == PG_OK ? search_ws_layout(d, dtype, turn_size(d, dtype, n, K), K, max_len).total : 0;
 }
 extern "C" int pg_beam_search(const pg_dims* d, int dtype, const float* params, const void* shadow, void* ws, size_t ws_bytes, int n,
                               int K, int max_len, const float* z, const uint8_t* allowed, double temp, uint8_t* tokens,
@@ -194,10 +204,16 @@ extern "C" int pg_beam_search(const pg_dims* d, int dtype, const float* params, 
   PG_TRY(check_search(d, dtype, n, K, max_len));
   PG_REQUIRE(params && shadow && ws && z && tokens && end_pads && scores, "pg_beam_search: NULL buffer");
   PG_REQUIRE(temp > 0.0 && isfinite(temp) && isfinite(2.0 / temp), "pg_beam_search: temperature must be positive and finite");
-  const size_t need = search_ws_layout(d, dtype, n, K, max_len).total;
+  const int m = turn_size(d, dtype, n, K);
+  const size_t need = search_ws_layout(d, dtype, m, K, max_len).total;
   if (ws_bytes < need) PG_FAIL(PG_ERR_WORKSPACE, "pg_beam_search: workspace too small (%zu < %zu)", ws_bytes, need);
   PG_TRY(check_persist());
   PG_TRY(shadow_join((hipStream_t)stream));
-  return dtype == PG_BF16 ? search_t<bf16_t>(d, dtype, params, shadow, ws, n, K, max_len, z, allowed, temp, tokens, end_pads, scores, (hipStream_t)stream)
-                          : search_t<float>(d, dtype, params, shadow, ws, n, K, max_len, z, allowed, temp, tokens, end_pads, scores, (hipStream_t)stream);
+  for (int r = 0; r < n; r += m) {
+    const auto search = dtype == PG_BF16 ? search_t<bf16_t> : search_t<float>;
+    const long row = (long)r * K;
+    PG_TRY(search(d, dtype, params, shadow, ws, std::min(m, n - r), K, max_len, z + (long)r * d->Dz, allowed, temp, tokens + row * max_len,
+                  end_pads + row, scores + row, (hipStream_t)stream));
+  }
+  return PG_OK;
 }
