@@ -229,9 +229,9 @@ PG_API int pg_beam_search(const pg_dims* d, int dtype, const float* params, cons
 /* Pages of a cache of decoder states.  A cache is n_planes arrays ("planes", e.g. the fp32 state and the operand copy of every
  * layer); page p is row p of every plane: `bytes` bytes at base + p * pitch.  Any width, pitch and alignment is taken; planes
  * of one call may interleave in one buffer but not share bytes, and neither may parents, index, live, count, map and the
- * workspace share bytes with pages that the call writes, or compaction's four with each other (all refused).  Indices live on
- * the device and are checked by the kernels: one that is out of range moves nothing.  Bytes outside the pages named are left as
- * they are. */
+ * workspace share bytes with pages that the call writes, or compaction's four with each other (all refused; so are planes of
+ * different pitches whose columns overlap in rows of the pitches' greatest common divisor).  Indices live on the device and
+ * are checked by the kernels: one that is out of range moves nothing.  Bytes outside the pages named are left as they are. */
 #define PG_MAX_PLANES 32
 typedef struct pg_plane {
   void* base;

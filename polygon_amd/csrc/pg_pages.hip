@@ -1,6 +1,7 @@
 // Pages of a cache of decoder states: reorder inside groups, fork, compaction.
 #include "pg_pages.h"
 #include "pg_host.h"
+#include <numeric>
 
 // What a move kernel needs of a cache: its planes, and how their columns are dealt out to waves.  A lane takes 16 bytes, so a wave
 // covers PG_SEG = 1024 bytes of one page, or - pages of at most 512 bytes - 64 / lanes neighbouring groups of pages at once
@@ -40,14 +41,16 @@ template <bool MIX> __host__ __device__ __forceinline__ long plane_units(const P
   return MIX ? (groups + 63) / 64 * pl.first[pl.n] : groups * (pl.first[pl.n] / 64);
 }
 
-// Two planes of `pages` pages share bytes: their spans overlap, unless they interleave with one pitch.
+// Two planes of na and nb pages share bytes (or, where their pitches differ, may: then only planes are told apart whose columns
+// differ in rows of the pitches' greatest common divisor, at which the pages of both recur).  A single page has no pitch.
 static bool planes_share(const pg_plane& a, long na, const pg_plane& b, long nb) {
   if (na < 1 || nb < 1) return false;
   const uintptr_t a0 = (uintptr_t)a.base, b0 = (uintptr_t)b.base;
   if (a0 + (na - 1) * a.pitch + a.bytes <= b0 || b0 + (nb - 1) * b.pitch + b.bytes <= a0) return false;
-  if (a.pitch != b.pitch) return true;
-  const long d = (long)((b0 >= a0 ? b0 - a0 : (uintptr_t)a.pitch - (a0 - b0) % a.pitch) % a.pitch);   // b's column relative to a's
-  return d < a.bytes || d + b.bytes > a.pitch;
+  const uintptr_t row = std::gcd(na > 1 ? a.pitch : 0, nb > 1 ? b.pitch : 0);
+  if (row == 0) return true;
+  const long d = (long)(b0 >= a0 ? (b0 - a0) % row : (row - (a0 - b0) % row) % row);   // b's column relative to a's
+  return d < a.bytes || d + b.bytes > (long)row;
 }
 static int check_planes(const char* who, const pg_plane* planes, int n_planes, long pages) {
   PG_REQUIRE(planes && n_planes >= 1 && n_planes <= PG_MAX_PLANES, "%s: %d planes outside [1,%d]", who, n_planes, PG_MAX_PLANES);
@@ -65,7 +68,7 @@ static int check_planes(const char* who, const pg_plane* planes, int n_planes, l
 // read the indices.
 static int check_apart(const char* who, const pg_plane* planes, int n_planes, long pages, const char* what, const void* at, long bytes) {
   for (int i = 0; i < n_planes; ++i)
-    PG_REQUIRE(!planes_share(planes[i], pages, pg_plane{(void*)at, planes[i].pitch, bytes}, bytes > 0), "%s: %s shares bytes with plane %d",
+    PG_REQUIRE(!planes_share(planes[i], pages, pg_plane{(void*)at, bytes, bytes}, bytes > 0), "%s: %s shares bytes with plane %d",
                who, what, i);
   return PG_OK;
 }

@@ -128,3 +128,51 @@ def test_workspace():
 def test_limits_match_the_header():
     text = open(os.path.join(os.path.dirname(__file__), "..", "include", "polygon_hip.h")).read()
     assert "#define PG_MAX_BEAMS %d\n" % beam.MAX_BEAMS in text and ctypes.sizeof(ctypes.c_long) == ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def _bytes_of(plane, pages):
+    base, pitch, width = plane
+    return {base + p * pitch + i for p in range(pages) for i in range(width)}
+
+
+def test_planes_of_different_pitches_are_told_from_shared_ones():
+    """columns of one buffer by rows, by every other row, or one row alone: refused where bytes are shared, and only there"""
+    L = beam._entries()
+    at = lambda row, col, step, width: (FAKE + row * 128 + col, step * 128, width)  # noqa: E731
+    one = lambda row, col, width: (FAKE + row * 128 + col, width, width)            # noqa: E731  (one page: the pitch says nothing)
+    apart = [(one(3, 64, 64), 1, at(0, 0, 1, 64), 8), (one(0, 64, 64), 1, at(0, 0, 1, 64), 8), (one(7, 0, 64), 1, at(0, 64, 1, 64), 8),
+             (one(3, 64, 16), 1, one(3, 0, 64), 1), (at(0, 64, 2, 64), 4, at(0, 0, 1, 64), 8), (at(0, 0, 2, 128), 4, at(1, 0, 2, 128), 4),
+             (at(0, 0, 2, 128), 4, at(1, 0, 4, 128), 2), (one(9, 0, 64), 1, at(0, 0, 1, 128), 8), (at(1, 32, 3, 32), 3, at(0, 64, 2, 64), 5)]
+    shared = [(one(3, 32, 64), 1, at(0, 0, 1, 64), 8), (one(3, 64, 65), 1, at(0, 0, 1, 64), 8), (one(3, 0, 64), 1, one(3, 63, 64), 1),
+              (at(0, 32, 2, 64), 4, at(0, 0, 1, 64), 8), (at(0, 0, 2, 128), 4, at(0, 0, 4, 128), 2), (at(1, 60, 3, 32), 3, at(0, 64, 2, 64), 5)]
+    for case, share in [(c, False) for c in apart] + [(c, True) for c in shared]:
+        a, na, b, nb = case
+        assert bool(_bytes_of(a, na) & _bytes_of(b, nb)) == share
+        for (d, nd), (s, ns) in (((a, na), (b, nb)), ((b, nb), (a, na))):
+            d, s = (d[0], d[1], min(d[2], s[2])), (s[0], s[1], min(d[2], s[2]))       # (a fork's planes have one width)
+            if bool(_bytes_of(d, nd) & _bytes_of(s, ns)) != share:
+                continue
+            assert L.pg_pages_fork(_pl(d), _pl(s), 1, nd, ns, None, None) == -1       # refused, or stops at the missing index
+            assert (b"share" if share else b"index is NULL") in L.pg_last_error(), case
+
+
+def test_planes_share_no_byte_by_counting():
+    """random planes: what shares a byte is always refused, whatever the pitches"""
+    import random
+    rng, L = random.Random(4), beam._entries()
+    refused = taken = 0
+    for _ in range(4000):
+        width = rng.randint(1, 40)
+        planes = []
+        for _ in range(2):
+            n = rng.choice([1, 1, 2, 3, 7])
+            planes.append(((FAKE + rng.randint(0, 200), max(width, rng.choice([16, 32, 48, 64, 96, 128, width, width + 5])), width), n))
+        (d, nd), (s, ns) = planes
+        status = L.pg_pages_fork(_pl(d), _pl(s), 1, nd, ns, None, None)
+        assert status == -1
+        if _bytes_of(d, nd) & _bytes_of(s, ns):
+            assert b"share" in L.pg_last_error()
+            refused += 1
+        else:
+            taken += b"index is NULL" in L.pg_last_error()
+    assert refused > 500 and taken > 500
