@@ -4,13 +4,15 @@ runs the whole decode; these serve a program that drives its own.
 
 All work is enqueued on the current stream of the tensors' device; nothing synchronises or copies to the host.  Arguments are
 checked on the host (shapes, types, devices, strides); indices are device data and checked by the kernels: one that is out of
-range moves nothing.  Nothing here is differentiable.
+range moves nothing.  Nothing here is differentiable; pages that move are tensors modified in place, and count as that for
+autograd: a backward pass that needs what they held raises.
 """
 import ctypes
 import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from polygon_amd import _lib
 
@@ -163,6 +165,7 @@ def reorder_pages(planes, parents):
         raise ValueError("parents %s does not name %d pages" % (list(shape), P))
     parents = _index(parents, dev, "parents")
     _call(dev, _entries().pg_pages_reorder, d, len(planes), shape[0], shape[1], parents.data_ptr())
+    increment_version(planes)
 
 
 def fork_pages(dst, src, index):
@@ -180,6 +183,7 @@ def fork_pages(dst, src, index):
         raise ValueError("index %s does not name a page for each of %d" % (list(index.shape), P))
     index = _index(index, dev, "index")
     _call(dev, _entries().pg_pages_fork, d, s, len(dst), P, Q, index.data_ptr())
+    increment_version(dst)
 
 
 def compact_pages(planes, live):
@@ -195,4 +199,5 @@ def compact_pages(planes, live):
     where, ws = count.new_empty(P), count.new_empty(need, dtype=torch.uint8) if need else None
     _call(dev, L.pg_pages_compact, d, len(planes), P, live.data_ptr(), count.data_ptr(), where.data_ptr(),
           None if ws is None else ws.data_ptr(), need)
+    increment_version(planes)
     return count, where
