@@ -137,6 +137,17 @@ class _Engine:
     def params(self):
         return list(self.model.vae.parameters())
 
+    def flat_in_place(self, ps):
+        """Whether the parameters are the views of ``flat`` that ensure_flat makes of them."""
+        if self.flat is None or self.flat.device != ps[0].device:
+            return False
+        off, base = 0, self.flat.data_ptr()
+        for p in ps:
+            if p.data_ptr() != base + 4 * off or p.dtype != torch.float32:
+                return False
+            off += p.numel()
+        return True
+
     def ensure_flat(self):
         """Makes the parameters (25 for the default shapes) views of one flat fp32 buffer in optimiser order (include/polygon_hip.h)."""
         m = self.model
@@ -146,15 +157,7 @@ class _Engine:
             raise _lib.PolygonHipError(
                 "polygon_amd.VAE computes only on an MI355X (`cuda`) device; the model is on %s. Move it with "
                 "model.to('cuda') -- there is no CPU path in this package." % dev)
-        ok = self.flat is not None and self.flat.device == dev
-        if ok:
-            off = 0
-            base = self.flat.data_ptr()
-            for p in ps:
-                if p.data_ptr() != base + 4 * off or p.dtype != torch.float32:
-                    ok = False
-                    break
-                off += p.numel()
+        ok = self.flat_in_place(ps)
         if not ok:
             for p in ps:
                 if p.dtype != torch.float32:
@@ -211,9 +214,24 @@ class _Engine:
     def invalidate(self):
         self.shadow_key = None
 
+    def shadow_now(self, ps):
+        return (self.flat.data_ptr(), self.dtype_code(), tuple(p._version for p in ps))
+
+    def check_capture(self, what):
+        """Raises if the current stream is being captured and the weights' operand copies are not up to date: the capture would
+        record their layout instead of running it, and later calls would take it for done."""
+        ps = self.params()
+        if ps[0].device.type != "cuda":
+            return                      # (refused by ensure_flat)
+        with torch.cuda.device(ps[0].device):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not (self.flat_in_place(ps) and self.shadow_now(ps) == self.shadow_key):
+            raise _lib.PolygonHipError("%s cannot be captured while the weights are new or changed since the last call: call it "
+                                       "once before the capture" % what)
+
     def ensure_shadow(self):
         flat = self.ensure_flat()
-        key = (flat.data_ptr(), self.dtype_code(), tuple(p._version for p in self.params()))
+        key = self.shadow_now(self.params())
         if key != self.shadow_key:
             L = _lib.lib()
             L.pg_shadow_bytes.restype = ctypes.c_size_t
@@ -783,12 +801,15 @@ class VAE(nn.Module):
 
     def beam_search_tokens(self, z, beam_width=8, max_len=100, temp=1.0, allowed=None):
         """Token form of ``beam_search``: (tokens uint8 [n, K, max_len], end_pads int32 [n, K], scores float32 [n, K]) on the
-        device, best hypothesis first.  Nothing is copied to the host or waited for."""
+        device, best hypothesis first.  Nothing is copied to the host or waited for, so a call can be captured into a graph,
+        if one with the present weights was made before (otherwise it raises).  Replays use the weights as the last call outside a
+        graph saw them; where parameters were moved to other memory since, capture again."""
         eng = self._engine
         K = int(beam_width)
         if z.dim() != 2 or z.shape[1] != self.d_z:
             raise RuntimeError("z must be [n, %d], got %s" % (self.d_z, list(z.shape)))
         n, V = z.shape[0], len(self.vocabulary)
+        eng.check_capture("beam search")
         dev = eng.ensure_flat().device
         with torch.no_grad(), torch.cuda.device(dev):
             eng.ensure_shadow()
