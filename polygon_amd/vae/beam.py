@@ -18,6 +18,7 @@ from polygon_amd import _lib
 
 MAX_BEAMS = 32      # PG_MAX_BEAMS
 NO_WORKSPACE_V = 1024     # up to here pg_beam_select_workspace_bytes is 0: not asked
+INT_END = 1 << 31         # the C entries' numbers are 32 bits wide, and ctypes drops what is above them
 
 
 class BeamStep(NamedTuple):
@@ -87,6 +88,8 @@ def beam_select(logits, scores, finished=None, mask=None, temp=1.0, eos=-1, pad=
     if scores.shape != (n, K) or scores.dtype != torch.float32 or scores.device != dev:
         raise ValueError("scores must be [%d, %d] float32 on %s, got %s %s on %s" % (n, K, dev, list(scores.shape), scores.dtype,
                                                                                   scores.device))
+    if not (-INT_END <= eos < INT_END and -INT_END <= pad < INT_END and n < INT_END and K < INT_END and V < INT_END):
+        raise ValueError("n=%d, K=%d, V=%d, eos=%d, pad=%d: not all fit 32 bits" % (n, K, V, eos, pad))
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
@@ -126,6 +129,8 @@ def _planes(planes, what):
         raise ValueError("%s: no planes" % what)
     shape, dev = planes[0].shape, planes[0].device
     P = shape[0] if shape else -1
+    if P >= INT_END:
+        raise ValueError("%s: %d pages, their number does not fit 32 bits" % (what, P))
     out = []
     for t in planes:
         shape = t.shape

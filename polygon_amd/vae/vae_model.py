@@ -808,7 +808,11 @@ class VAE(nn.Module):
         K = int(beam_width)
         if z.dim() != 2 or z.shape[1] != self.d_z:
             raise RuntimeError("z must be [n, %d], got %s" % (self.d_z, list(z.shape)))
-        n, V = z.shape[0], len(self.vocabulary)
+        n, V, max_len = z.shape[0], len(self.vocabulary), int(max_len)
+        if not 1 <= K <= MAX_BEAMS:
+            raise RuntimeError("beam_width must lie in [1, %d], got %d" % (MAX_BEAMS, K))
+        if not 2 <= max_len <= 1 << 20:
+            raise RuntimeError("max_len must lie in [2, 2^20], got %d" % max_len)
         eng.check_capture("beam search")
         dev = eng.ensure_flat().device
         with torch.no_grad(), torch.cuda.device(dev):
@@ -818,8 +822,6 @@ class VAE(nn.Module):
                 if tuple(allowed.shape) != (V,):
                     raise RuntimeError("allowed must have shape [%d]" % V)
                 allowed = (allowed != 0).to(dev, torch.uint8).contiguous()
-            if not 1 <= K <= MAX_BEAMS:
-                raise RuntimeError("beam_width must lie in [1, %d], got %d" % (MAX_BEAMS, K))
             L = _lib.lib()
             L.pg_beam_search_workspace_bytes.restype = ctypes.c_size_t
             tokens = torch.empty(n, K, max_len, dtype=torch.uint8, device=dev)
@@ -828,12 +830,12 @@ class VAE(nn.Module):
             CH = max(1, 65536 // K)      # latents per library call: bounds the workspace (~14 KB per beam) whatever n is
             for r0 in range(0, n, CH):
                 m = min(CH, n - r0)
-                nbytes = L.pg_beam_search_workspace_bytes(ctypes.byref(eng.dims), eng.dtype_code(), m, K, int(max_len))
+                nbytes = L.pg_beam_search_workspace_bytes(ctypes.byref(eng.dims), eng.dtype_code(), m, K, max_len)
                 if nbytes == 0:
                     raise _lib.PolygonHipError("pg_beam_search_workspace_bytes: " + L.pg_last_error().decode())
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
                 _lib.check(L.pg_beam_search(ctypes.byref(eng.dims), eng.dtype_code(), _lib.ptr(eng.flat), _lib.ptr(eng.shadow),
-                                            _lib.ptr(ws), ctypes.c_size_t(nbytes), m, K, int(max_len), _lib.ptr(z[r0:r0 + m]),
+                                            _lib.ptr(ws), ctypes.c_size_t(nbytes), m, K, max_len, _lib.ptr(z[r0:r0 + m]),
                                             _lib.ptr(allowed), ctypes.c_double(float(temp)), _lib.ptr(tokens[r0:r0 + m]),
                                             _lib.ptr(end_pads[r0:r0 + m]), _lib.ptr(scores[r0:r0 + m]), _lib.stream_ptr()),
                            "pg_beam_search")

@@ -176,3 +176,25 @@ def test_planes_share_no_byte_by_counting():
         else:
             taken += b"index is NULL" in L.pg_last_error()
     assert refused > 500 and taken > 500
+
+
+def test_wrappers_refuse_what_the_entries_integers_do_not_hold():
+    """the C entries count in 32 bits: a larger number must not reach them as what is left of it"""
+    x, s = torch.zeros(2, 3, 5), torch.zeros(2, 3)
+    for kw in (dict(eos=1 << 32), dict(eos=-(1 << 32) + 2), dict(pad=1 << 32), dict(pad=(1 << 32) + 1)):
+        with pytest.raises(ValueError, match="32 bits"):
+            vae.beam_select(x, s, **kw)
+    meta = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device="meta")  # noqa: E731
+    many = (1 << 32) + 1
+    for n, K, V in ((many, 1, 1), (1, many, 1), (1, 1, many)):
+        with pytest.raises(ValueError, match="32 bits"):
+            vae.beam_select(meta(n, K, V), meta(n, K))
+    pages, index = meta(many, 4), meta(many, dtype=torch.int32)
+    with pytest.raises(ValueError, match="32 bits"):
+        vae.reorder_pages([pages], index.view(many, 1))
+    with pytest.raises(ValueError, match="32 bits"):
+        vae.fork_pages([pages], [meta(3, 4)], index)
+    with pytest.raises(ValueError, match="32 bits"):
+        vae.fork_pages([meta(3, 4)], [pages], meta(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="32 bits"):
+        vae.compact_pages([pages], meta(many, dtype=torch.bool))

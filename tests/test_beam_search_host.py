@@ -42,3 +42,16 @@ def test_latents_beyond_the_cells_reach_are_taken_in_turn(Hd, Dz, K, dtype, es):
 def test_a_latent_that_no_call_could_decode_is_refused():
     assert _bytes(_dims(1 << 24, 8, L=1), _lib.PG_F32, 1, 32) == 0 and b"2 GiB" in _lib.lib().pg_last_error()
     assert _bytes(_dims(1 << 20, 8, L=1), _lib.PG_F32, 1, 32) > 0
+
+
+def test_search_checks_its_numbers_before_anything_is_allocated():
+    """(a max_len that 32 bits do not hold would fill its tensors' first columns only)"""
+    import torch
+    from polygon_amd.vae.vae_model import VAE
+    model, z = VAE(q_d_h=32, d_z=16, d_d_h=32, d_n_layers=1), torch.zeros(0, 16)
+    for max_len in ((1 << 32) + 5, (1 << 20) + 1, 1, -3):
+        with pytest.raises(RuntimeError, match="max_len"):
+            model.beam_search_tokens(z, 4, max_len)
+    for width in (0, 33, (1 << 32) + 1):
+        with pytest.raises(RuntimeError, match="beam_width"):
+            model.beam_search_tokens(z, width, 9)
