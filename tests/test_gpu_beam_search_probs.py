@@ -111,3 +111,30 @@ def test_search_over_the_samplers_probabilities(dims, symbols, K, n, T, dt):
     tok, end, sc = [t.cpu().numpy() for t in model.beam_search_tokens(z, K, T)]
     assert sure.sum() >= 3 and end[sure].max() >= 4, "too few of the searches are clearly decided"
     assert np.array_equal(tok[sure], strings[sure]) and (np.abs(sc[sure] - s[sure]) <= room[sure]).all()
+
+
+SHAPES = [(dict(Hq=32, Dz=8, Hd=32, L=1), 0), (dict(Hq=32, Dz=24, Hd=96, L=2), 0), (dict(Hq=64, Dz=40, Hd=160, L=8), 0),
+          (dict(Hq=32, Dz=8, Hd=32, L=2), 100), (dict(Hq=32, Dz=16, Hd=224, L=4), 66), (dict(Hq=32, Dz=16, Hd=64, L=1), 5)]
+
+
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("dims,symbols", SHAPES)
+def test_decoder_shapes(dims, symbols, dt):
+    """hidden sizes that no tile divides, one layer to eight, a vocabulary of five; one beam and as many as there are"""
+    model = make_model(dims, symbols, dt, 2.0, 0.5)
+    for K, n, T in ((1, 70, 20), (7, 33, 19), (32, 5, 10)):
+        z = torch.randn(n, dims["Dz"], generator=torch.Generator().manual_seed(K)).cuda()
+        tok, end, sc = model.beam_search_tokens(z, K, T)
+        lp = log_probs(model, z.repeat_interleave(K, 0), tok.view(n * K, T))
+        tok, end, sc = tok.view(n * K, T).cpu().numpy().astype(int), end.view(-1).cpu().numpy(), sc.view(-1).double().cpu().numpy()
+        tol, want, room, rows = step_tolerance(model), np.zeros(n * K), np.zeros(n * K), np.arange(n * K)
+        assert np.isfinite(sc).all() or symbols == 5
+        for i in range(1, T):
+            inside = i < end
+            step = np.where(inside, lp[i - 1, rows, tok[:, i]], 0.0)
+            want += step
+            room += np.where(inside, tol(want, step), 0.0)
+        has = np.isfinite(sc)
+        assert (np.abs(sc - want)[has] <= room[has]).all(), (K, float(np.abs(sc - want)[has].max()))
+        assert (end[~has] == 0).all()
+        assert all(len({tuple(t) for t, e in zip(tok[g * K:g * K + K], end[g * K:]) if e}) == has[g * K:g * K + K].sum() for g in range(n))
