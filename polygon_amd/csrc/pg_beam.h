@@ -46,7 +46,8 @@ __device__ __forceinline__ float beam_key_number(unsigned long long k) { return 
 // 2^t of t <= 0 in 64 bits: t = n + f with |f| <= 1/2 (adding 1.5 * 2^52 leaves n in the low bits), 2^f = 1 + f q(f) with q fitted
 // to the least largest relative error of 2^f on that interval, 8.1e-13 (Lawson's iteration), n added to the exponent.  13
 // instructions, all at the full 64-bit rate, which is also that of fp32 here.  Which candidate wins hangs on the normaliser:
-// 32 bits (6e-8) would let near ties flip, 8e-13 is a millionth of what a score's rounding to fp32 can tell.  2^0 is exactly 1.
+// 32 bits (6e-8) would let near ties flip; 8e-13 is a 70000th of what a score near 1 is rounded by (2^-24), less beside larger ones.
+// 2^0 is exactly 1.
 typedef __attribute__((ext_vector_type(2))) unsigned u32x2;
 constexpr double BEAM_LOG2E = 1.4426950408889634074;
 __device__ __forceinline__ double beam_exp2(double t) {

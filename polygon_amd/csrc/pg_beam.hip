@@ -10,7 +10,8 @@
 // group takes the G waves that its K rows need.  The logits are read once and stay in registers (at most 32 of them), and
 // softmax's reductions stay inside a wave (for N = 16 inside DPP rows).  With G > 1 the first wave selects from the G waves'
 // few best.  Bound by instructions (some 700 a wave at 8 x 51, half of them the selection, a fifth the 64-bit exponentials):
-// 8192 x 8 x 51 fp32 14.4 us for 10.5 MB, 1024 x 32 x 128 bf16 with masks 18.8 us, one group 4.6 us, most of it latency.
+// 8192 x 8 x 51 fp32 14.5 us for 10.5 MB, 1024 x 32 x 128 bf16 with masks 19.0 us, one group 4.4 us, most of it latency (each launch
+// by itself; back to back a call of 8192 x 8 x 51 takes 12.5).
 // Measured against the chunked kernels below where those could start: 4096 x 8 x 129 19 us here, 63 there; 2000 x 8 x 1000 28 and 56.
 constexpr int SW = 4;      // waves per workgroup, where G is not more
 template <int W, int ROWS> struct ShortLds {
@@ -128,7 +129,9 @@ __global__ __launch_bounds__(64 * (G > SW ? G : SW)) void beam_select_short_kern
 // groups that fit 32 rows (one tile of the matrix instruction); its four waves contract every fourth step of H each,
 // straight from memory (the weights, 64 KB in bf16, stay in the L2s), their partial logits meet in LDS, and the selection reads
 // them there.  For few rows it is bound by latency: 9.4 us for one group where the tiled product and the selection took 8.7 and
-// 4.5; 11 instead of 15.4 + 7.2 us at 512 rows, 49 instead of 25 + 13 at 65536 (where the cells take 1500).
+// 4.5; 11 instead of 15.4 + 7.2 us at 512 rows.  At 65536 rows it takes 49 instead of 25 + 13; used there too: those 11 us are 0.7 % of a
+// step (the cells take 1510), rows shrink as molecules leave (median over a search of 65536 rows: 27 us), and a second path would
+// serve only a search's first steps.
 template <typename T, int E, int P, int G>
 __global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTrack tr, const T* __restrict__ h, int H,
                                                             const T* __restrict__ fcw, const float* __restrict__ fcb) {
@@ -188,8 +191,8 @@ __global__ __launch_bounds__(64 * SW) void beam_head_kernel(BeamSelect a, BeamTr
 // groups, many chunks), a workgroup per row first merges the row's chunks into one.
 // 64 x 8 x 131072 fp32 (268 MB): 73.7 us, 3.6 TB/s, and 7.0 us for the join.  Reading alone takes 44 us; the exponentials add 26
 // (17 instructions a symbol; matrix units do not help an exponential), the later tiles' selection 13: the vector units are busy
-// 70 % of the time.  No gain: tiles of 32 symbols a lane (87 us: fewer waves), the next tile loaded ahead into registers (77)
-// or through LDS (70.5), more or fewer waves.
+// 70 % of the time.  Not kept: tiles of 32 symbols a lane (87 us: fewer waves), the next tile loaded ahead into registers (77), or
+// through LDS (70.5: some 3 %, for aligned rows only, and a second variant of the loop); more or fewer waves gain nothing.
 constexpr int LE = 16, TILE = 64 * LE, LONG_KEYS = PG_MAX_BEAMS + 1;
 struct BeamChunk {
   double sum;
@@ -497,6 +500,9 @@ __global__ __launch_bounds__(64 * JW) void beam_join_kernel(BeamSelect a, BeamLo
   // score: then the lower index counts.  What a list left out can only matter if its last entry, the K + 1st, still has the score of
   // the group's last winner (it cannot have a better one: K others of the list are as good) and a lower logit could have it too;
   // such a chunk is read again for the symbols of that score.  (Logits that tie by being equal are listed by index already.)
+  // That is at most one chunk of a group, read up to K times by this workgroup alone - slow where a merged row, which is one chunk,
+  // has one score all over.  All logits zero, fp32, against ordinary ones: 4 x 8 x 32001 53 and 17 us, 64 x 8 x 131072 232 and 81,
+  // 1 x 8 x 131072 861 and 20, 1 x 32 x 131072 3490 and 40, 1 x 32 x 2^20 26300 and 78.
   const unsigned edge = (unsigned)(won[K - 1] >> 32);
   if (edge == 0) {
     if (wave == 0) beam_write<false>(a, BeamTrack{}, g, g, won, fin, place, lane);
@@ -604,7 +610,8 @@ template <class F> static void with_waves(int K, int rows, F f) {
   else if (K <= 8 * rows) f(Int<8>{});
   else f(Int<16>{});
 }
-// f(N, E, P, G): the narrowest kernel that holds V symbols and K beams
+// f(N, E, P, G): the narrowest kernel that holds V symbols and K beams.  Up to 4 beams one row per 16 lanes (P = 1) instead of two:
+// 8192 groups of 4 x 51 8.3 us against 10.0, 65536 of 4 x 128 57 against 78, one of 1 x 51 3.5 against 3.9.
 template <class F> static void with_short_shape(int V, int K, F f) {
   auto shape = [&](auto n, auto e, auto p) { with_waves(K, 64 / n * p, [&](auto g) { if constexpr (g * (64 / n * p) <= PG_MAX_BEAMS) f(n, e, p, g); }); };
   if (V <= 64) K <= 4 ? f(Int<16>{}, Int<4>{}, Int<1>{}, Int<1>{}) : shape(Int<16>{}, Int<4>{}, Int<2>{});

@@ -17,7 +17,7 @@ int shadow_join(hipStream_t st);   // pg_vae.hip
 
 // A compaction costs one launch of 6 us and the moves of what closes up; a step of the default decoder takes 60 us for a few
 // rows and 1.6 ms for 65536.  Whole searches, 99 steps of the bf16 default decoder: 1 latent x 5 beams 2.0 ms, 64 x 8 6.1 ms,
-// 1024 x 8 12.3 ms, 8192 x 8 77.6 ms (72 of them the cells, 2.8 projection and selection, 2.2 reorder, 0.1 compaction).
+// 1024 x 8 12.3 ms, 8192 x 8 77.6 ms (72.1 of them the cells, 2.9 projection and selection, 2.4 reorder, 0.1 compaction).
 constexpr int COMPACT_EVERY = 8;
 
 // Latents of one turn.  The cells and the products read states and latents by 32-bit byte offsets into a descriptor of 2 GiB, and

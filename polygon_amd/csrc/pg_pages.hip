@@ -35,8 +35,9 @@ static bool any_narrow(const Planes& pl) {
   return false;
 }
 // MIX: some planes are narrow, and units are dealt out in blocks of 64 groups.  Otherwise group by group, with less arithmetic and
-// fewer registers per wave (measured with 9 KB pages, all wide: 77 us so, 95 us in blocks; with pages of 64 and 128 bytes a wave
-// per group and plane took 146 us, blocks 65).
+// fewer registers per wave.  Three planes of 2 KB and three of 1 KB, all wide, in blocks instead: reorder of 8192 groups of 4 56.5 us
+// against 50.3, compaction of 8192 pages of 8 such rows 59.6 against 52.9.  Pages of 64 and 128 bytes by a wave per group and plane
+// instead: reorder of 8192 groups of 8 11.4 us against 5.1; of 512 and 256 bytes 13.2 against 10.2 (64 groups: 3.8 against 4.4).
 template <bool MIX> __host__ __device__ __forceinline__ long plane_units(const Planes& pl, long groups) {
   return MIX ? (groups + 63) / 64 * pl.first[pl.n] : groups * (pl.first[pl.n] / 64);
 }
@@ -246,8 +247,10 @@ static int compact_grid(const Planes& pl, bool mix, long n) {
 }
 
 // Up to PLAN_PAGES pages: ONE launch, every workgroup works the plan out for itself (n flag bytes from L2, a scan, the moves'
-// ends as 16-bit lists in LDS) and takes its share of the moves.  8192 pages of 72 KB, half live (302 MB): 68 us, 4.4 TB/s, some
+// ends as 16-bit lists in LDS) and takes its share of the moves.  8192 pages of 72 KB, half live (302 MB): 66 us, 4.5 TB/s, some
 // 5 us of it the plan; 64 pages 7 us.  Units in flight per wave (MV) 8: 76 us; 1024 or 4096 workgroups 72 and 76.
+// 16384 is as many flags as 256 threads hold in 64 bits each, and up to there this is the faster way: pages of 2 KB, half live, 300
+// pages 5.8 us against 9.4 with the plan in a launch of its own, 4096 pages 6.7 and 9.6, 16384 pages 12.8 and 19.7.
 constexpr int PLAN_PAGES = 16384;
 template <bool MIX>
 __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, const int* __restrict__ n_dev,
@@ -293,7 +296,8 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(Planes pl, int n, co
   move_pages<MIX>(pl, moves, hole, mover);
 }
 
-// More pages: the plan by one workgroup into the workspace, then the moves.
+// More pages: the plan by one workgroup into the workspace, then the moves.  Bound by that workgroup's walk through the flags: pages of
+// 4 bytes, half live, 65536 of them 61 us, 300000 267 us, a million 1.02 ms (pages of 2 KB: 66, 344 us and 1.31 ms).
 __global__ __launch_bounds__(1024) void pages_plan_kernel(int n, const int* __restrict__ n_dev,
                                                           const uint8_t* __restrict__ live, int32_t* __restrict__ count,
                                                           int32_t* __restrict__ map, int32_t* __restrict__ moves,
