@@ -802,8 +802,9 @@ class VAE(nn.Module):
     def beam_search_tokens(self, z, beam_width=8, max_len=100, temp=1.0, allowed=None):
         """Token form of ``beam_search``: (tokens uint8 [n, K, max_len], end_pads int32 [n, K], scores float32 [n, K]) on the
         device, best hypothesis first.  Nothing is copied to the host or waited for, so a call can be captured into a graph,
-        if one with the present weights was made before (otherwise it raises).  Replays use the weights as the last call outside a
-        graph saw them; where parameters were moved to other memory since, capture again."""
+        if one with the present weights was made before (otherwise it raises).  Replays read the operand copies that the last call
+        outside a graph laid out: after a change of the weights, call before the next replay, and capture again where parameters
+        were moved to other memory."""
         eng = self._engine
         K = int(beam_width)
         if z.dim() != 2 or z.shape[1] != self.d_z:
